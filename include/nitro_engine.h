@@ -297,6 +297,119 @@ int nr_paged_attention_decode_static(const float* q, const float* kpool, const f
 int nr_q8_matmul(const float* x, const int8_t* q, const float* scales, float* out,
                  int32_t M, int32_t N, int32_t K, int32_t q8_mode, void* stream);
 
+/* ------------------------------------------------------------------ 8-bit K/V pages
+ * No counterpart in the reference, whose pages are fp32.  Device pointers and `stream` as
+ * above, asynchronous, no allocation and no host synchronisation, so every call can be
+ * captured into a CUDA graph (make the first call on each device outside a capture).  Each
+ * call runs on the current device, which must be the stream's.  Sums, softmax statistics
+ * and rotations are fp32; 16-bit outputs are rounded once.
+ *
+ * Element type of the q, k, v, logits and attention outputs of these entry points. */
+#define NR_DTYPE_F32   0
+#define NR_DTYPE_BF16  1
+#define NR_DTYPE_F16   2
+
+/* Value written to *error_flag (if not NULL; first writer wins, never cleared by a call) by
+ * the entry points below: 2 = a length, position or page id out of range (each entry point
+ * says what it does then), 1 = a bounded device-side wait gave up. */
+
+/* Pages of 16 tokens: codes [n_pages][n_layers][n_kv_heads][16][head_dim] in e4m3 (the
+ * OCP 8-bit format, largest value 448), with one fp32 scale per block of 16 tokens and head,
+ * [n_pages][n_layers][n_kv_heads]; value = code * scale.  head_dim 64 or 128.  codes 16-byte
+ * aligned. */
+typedef struct nr_kv8_pool {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t n_pages, n_layers, n_kv_heads, head_dim;
+} nr_kv8_pool;
+
+/* Pairs that a rotation turns: elements (2i, 2i+1) of the first rot_dim (the layout of
+ * src/model_q8.cpp:451-484), or (i, i + rot_dim/2). */
+#define NR_ROPE_INTERLEAVED 0
+#define NR_ROPE_HALF        1
+
+/* New tokens of B sequences, packed: rows cu_seqlens[b] .. cu_seqlens[b+1]-1 are the tokens
+ * of sequence b at positions start_pos[b], start_pos[b]+1, ...  Rows from cu_seqlens[B] to
+ * T-1 are padding: neither read nor written. */
+typedef struct nr_kv8_append_args {
+    const void* q;              /* [T] rows of n_heads*head_dim, or NULL                         */
+    const void* k;              /* [T] rows of n_kv_heads*head_dim                               */
+    const void* v;
+    void* q_out;                /* rotated q (may be q itself); NULL only if q is                */
+    void* k_out;                /* rotated k (may be k itself), or NULL                          */
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;  /* row strides in elements */
+    const int32_t* cu_seqlens;  /* [B+1], not decreasing, cu_seqlens[B] <= T                     */
+    const int32_t* start_pos;   /* [B]                                                           */
+    const int32_t* block_tables;/* [B][max_pages]                                                */
+    const float* rope_cos;      /* [rope_len][rot_dim/2], NULL if rot_dim is 0                   */
+    const float* rope_sin;
+    int32_t dtype;              /* NR_DTYPE_* of q, k, v, q_out, k_out                           */
+    int32_t B, T, n_heads, max_pages, layer;
+    int32_t rope_len;           /* rows of the tables                                            */
+    int32_t rot_dim;            /* first elements of a head that are rotated: 0, 16, 32 .. head_dim */
+    int32_t rope_layout;        /* NR_ROPE_*                                                     */
+} nr_kv8_append_args;
+
+/* Rotate q and k, write them out and append k (rotated) and v to the pages.  Each (page,
+ * head) block that gets tokens takes the smallest power of two 2^e >= 2^-126 with
+ * |x| <= 448 * 2^e for its new values as scale, or keeps the one it has where it holds
+ * tokens of this sequence already (start_pos not a multiple of 16) and its scale is larger.  Where the
+ * scale grows, the older tokens' codes are divided by the growth, exact but for values
+ * that fall below e4m3's normal range.  codes = round-to-nearest-even(x / scale); the
+ * rotation is two fp32 products and one fp32 sum per element, each rounded.  A block given a
+ * non-finite value gets a NaN scale, so that attention over it gives NaN.  Codes behind a
+ * sequence's last token are left as they were.
+ * No two sequences of a call may append to the same page.  A sequence whose rows, positions
+ * (up to max_pages*16, and rope_len if rot_dim > 0) are out of range is skipped, and so is
+ * the append of a page id outside [0, n_pages); both set *error_flag to 2.
+ * q, k, v, q_out, k_out and strides must be 16-byte aligned; outputs may equal their input
+ * (same stride) and overlap nothing else. */
+int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* args, int32_t* error_flag, void* stream);
+
+/* Decode paged attention for one layer over the 8-bit pages: nr_paged_attention_decode with
+ * q, out [B][n_heads*head_dim] of type `dtype`.  ctx_lens[b] in [0, max_pages*16]; a length
+ * of 0 gives a zero row.  Nothing behind a context's last token is used, whatever it holds.  A length
+ * out of range is clamped, a page id outside [0, n_pages) counts as 16 absent tokens; both
+ * set *error_flag to 2.  n_heads <= 16 * n_kv_heads.  q, out and workspace 16-byte aligned.
+ * workspace: nr_paged_attention_kv8_workspace_size() bytes, zero before the first call (each
+ * call leaves its counters zero again); calls that may overlap on the device need one each. */
+size_t nr_paged_attention_kv8_workspace_size(int32_t B, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                             int32_t max_pages);
+int nr_paged_attention_decode_kv8(const void* q, int32_t dtype, const nr_kv8_pool* pool, int32_t layer,
+                                  const int32_t* block_tables, int32_t max_pages, const int32_t* ctx_lens,
+                                  int32_t B, int32_t n_heads, void* out, void* workspace, int32_t* error_flag,
+                                  void* stream);
+
+/* Causal attention over whole prompts: B sequences packed in rows, q rows cu_q[b] ..
+ * cu_q[b+1]-1 against k, v rows cu_k[b] .. cu_k[b+1]-1 (cu_k NULL: cu_q).  The last query of
+ * a sequence sees all its keys, each earlier one a key less; a query that sees none gives a
+ * zero row.  q, out rows hold n_heads*head_dim elements, k, v rows n_kv_heads*head_dim, at
+ * the given row strides (in elements); scores are scaled by 1/sqrt(head_dim).  dtype
+ * NR_DTYPE_BF16 or NR_DTYPE_F16; head_dim 64 or 128.  Tq, Tk: rows of q (and out) and of
+ * k, v.  Rows outside every sequence are neither used (whatever they hold) nor written; a
+ * sequence's own k and v must be finite (a NaN or infinity reaches its earlier rows too).  A
+ * sequence whose rows are out of range is skipped and sets *error_flag to 2.  Pointers and
+ * strides 16-byte aligned; out overlaps none of the inputs. */
+int nr_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                        int64_t v_stride, void* out, int64_t out_stride, int32_t dtype, const int32_t* cu_q,
+                        const int32_t* cu_k, int32_t B, int32_t Tq, int32_t Tk, int32_t n_heads,
+                        int32_t n_kv_heads, int32_t head_dim, int32_t* error_flag, void* stream);
+
+/* Log probabilities from logits [M] rows of V (row stride in elements, any alignment of the
+ * type): target_logprob[m] = log softmax(row)[targets[m]] (NaN for a target outside
+ * [0, V)), entropy[m] = -sum p log p in nats, and the top_k largest logits' ids and log
+ * probabilities, largest first, equal logits by smaller id (top_k <= 32, <= V).  targets and
+ * target_logprob may both be NULL, entropy may be NULL, and the top arrays are NULL where
+ * top_k is 0.  -inf logits have probability 0 and add nothing to the entropy; a row that
+ * holds a NaN or +inf, or -inf throughout, gives NaN statistics; in the top list NaN ranks
+ * below -inf. */
+#define NR_LOGPROBS_MAX_TOP 32
+int nr_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int32_t M, int32_t V,
+                      const int32_t* targets, int32_t top_k, float* target_logprob, float* entropy,
+                      float* top_logprob, int32_t* top_ids, void* stream);
+
 /* ------------------------------------------------------------------ Q8_0 quantizer
  * scripts/quantize.py (quantize_q8, :7-23) byte for byte: per 32 consecutive weights (the
  * last block of a tensor may be shorter) scale = max|w| / 127 in fp32 (1e-9 for an

@@ -22,6 +22,12 @@ NR_SCHED_REFERENCE = 0
 NR_SCHED_PACKED = 1
 NR_KV_F32 = 0
 NR_KV_BF16 = 1
+NR_DTYPE_F32 = 0
+NR_DTYPE_BF16 = 1
+NR_DTYPE_F16 = 2
+NR_ROPE_INTERLEAVED = 0
+NR_ROPE_HALF = 1
+NR_LOGPROBS_MAX_TOP = 32
 
 
 class EngineLibraryMissing(RuntimeError):
@@ -61,6 +67,24 @@ class NrPlan(C.Structure):
 class NrStats(C.Structure):
     _fields_ = [("steps", C.c_int64), ("prefill_tokens", C.c_int64), ("decode_tokens", C.c_int64),
                 ("cache_hit_pages", C.c_int64), ("evictions", C.c_int64), ("kernel_launches", C.c_int64)]
+
+
+class NrKv8Pool(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("n_pages", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+    ]
+
+
+class NrKv8AppendArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p),
+        ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+        ("k_out_stride", C.c_int64), ("cu_seqlens", C.c_void_p), ("start_pos", C.c_void_p),
+        ("block_tables", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
+        ("dtype", C.c_int32), ("B", C.c_int32), ("T", C.c_int32), ("n_heads", C.c_int32), ("max_pages", C.c_int32),
+        ("layer", C.c_int32), ("rope_len", C.c_int32), ("rot_dim", C.c_int32), ("rope_layout", C.c_int32),
+    ]
 
 
 P = C.c_void_p
@@ -124,6 +148,12 @@ SIGNATURES = {
     "nr_paged_attention_decode": (C.c_int, [P, P, P, P, I32, P, I32, I32, I32, I32, I32, I32, P, P, P, P]),
     "nr_paged_attention_decode_static": (C.c_int, [P, P, P, P, I32, P, I32, I32, I32, I32, I32, I32, P, P, P]),
     "nr_q8_matmul": (C.c_int, [P, P, P, P, I32, I32, I32, I32, P]),
+    "nr_kv8_append": (C.c_int, [C.POINTER(NrKv8Pool), C.POINTER(NrKv8AppendArgs), P, P]),
+    "nr_paged_attention_kv8_workspace_size": (C.c_size_t, [I32, I32, I32, I32, I32]),
+    "nr_paged_attention_decode_kv8": (C.c_int, [P, I32, C.POINTER(NrKv8Pool), I32, P, I32, P, I32, I32, P, P, P, P]),
+    "nr_prompt_attention": (C.c_int, [P, C.c_int64, P, C.c_int64, P, C.c_int64, P, C.c_int64, I32, P, P, I32, I32,
+                                      I32, I32, I32, I32, P, P]),
+    "nr_token_logprobs": (C.c_int, [P, I32, C.c_int64, I32, I32, P, I32, P, P, P, P, P]),
     "nr_q8_quantized_size": (C.c_size_t, [C.c_int64]),
     "nr_quantize_q8_device": (C.c_int, [P, C.c_int64, P, P]),
     "nr_quantize_q8": (C.c_int, [P, C.c_int64, P, I32]),

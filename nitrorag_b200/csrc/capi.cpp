@@ -11,6 +11,7 @@
 
 #include "../../include/nitro_engine.h"
 #include "engine.h"
+#include "kv8.h"
 
 using nitro::Engine;
 using nitro::Request;
@@ -657,6 +658,110 @@ int nr_q8_matmul(const float* x, const int8_t* q, const float* scales, float* ou
     e.kind = nitro::kEpiStore; e.out = out; e.ldo = N;
     nitro::launch_gemm(g, e, (cudaStream_t)stream);
     return cudaGetLastError() == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+}
+
+static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// The pool fields every call checks; *out is the kernels' view of it.
+static bool read_kv8_pool(const nr_kv8_pool* p, int32_t layer, nitro::Kv8Pool* out) {
+    if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale || !aligned16(p->k) || !aligned16(p->v)) return false;
+    if (p->n_pages <= 0 || p->n_layers <= 0 || p->n_kv_heads <= 0 || layer < 0 || layer >= p->n_layers) return false;
+    if (p->head_dim != 64 && p->head_dim != 128) return false;
+    out->k = (uint8_t*)p->k; out->v = (uint8_t*)p->v; out->k_scale = p->k_scale; out->v_scale = p->v_scale;
+    out->n_pages = p->n_pages; out->n_layers = p->n_layers; out->n_kv_heads = p->n_kv_heads; out->head_dim = p->head_dim;
+    return true;
+}
+
+static bool valid_dtype(int32_t dtype) { return dtype == NR_DTYPE_F32 || dtype == NR_DTYPE_BF16 || dtype == NR_DTYPE_F16; }
+
+// Rows of `width` elements at a stride that keeps each row 16-byte aligned.
+static bool valid_rows(const void* p, int64_t stride, int64_t width, int32_t dtype) {
+    return p && aligned16(p) && stride >= width && stride * nitro::dtype_bytes(dtype) % 16 == 0;
+}
+
+int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* g, int32_t* error_flag, void* stream) {
+    nitro::Kv8AppendArgs a;
+    if (!g || !read_kv8_pool(pool, g->layer, &a.pool) || !valid_dtype(g->dtype)) return NR_ERR_INVALID;
+    if (!g->cu_seqlens || !g->start_pos || !g->block_tables || g->B <= 0 || g->B > 1024 || g->T <= 0 || g->max_pages <= 0)
+        return NR_ERR_INVALID;
+    const int hd = pool->head_dim;
+    const int64_t kw = (int64_t)pool->n_kv_heads * hd, qw = (int64_t)g->n_heads * hd;
+    if (!valid_rows(g->k, g->k_stride, kw, g->dtype) || !valid_rows(g->v, g->v_stride, kw, g->dtype)) return NR_ERR_INVALID;
+    if (g->k_out && !valid_rows(g->k_out, g->k_out_stride, kw, g->dtype)) return NR_ERR_INVALID;
+    if (!g->q != !g->q_out) return NR_ERR_INVALID;
+    if (g->q && (g->n_heads <= 0 || g->n_heads > (1 << 16) || !valid_rows(g->q, g->q_stride, qw, g->dtype) ||
+                 !valid_rows(g->q_out, g->q_out_stride, qw, g->dtype)))
+        return NR_ERR_INVALID;
+    if (pool->n_kv_heads > (1 << 16)) return NR_ERR_INVALID;
+    if ((g->q_out && g->q_out == g->q && g->q_out_stride != g->q_stride) ||
+        (g->k_out && g->k_out == g->k && g->k_out_stride != g->k_stride))
+        return NR_ERR_INVALID;
+    if (g->rot_dim < 0 || g->rot_dim > hd || g->rot_dim % 16) return NR_ERR_INVALID;
+    if (g->rope_layout != NR_ROPE_INTERLEAVED && g->rope_layout != NR_ROPE_HALF) return NR_ERR_INVALID;
+    if (g->rot_dim && (!g->rope_cos || !g->rope_sin || !aligned16(g->rope_cos) || !aligned16(g->rope_sin) || g->rope_len <= 0))
+        return NR_ERR_INVALID;
+    a.q = g->q; a.k = g->k; a.v = g->v; a.q_out = g->q_out; a.k_out = g->k_out;
+    a.q_stride = g->q_stride; a.k_stride = g->k_stride; a.v_stride = g->v_stride;
+    a.q_out_stride = g->q_out_stride; a.k_out_stride = g->k_out_stride;
+    a.cu_seqlens = g->cu_seqlens; a.start_pos = g->start_pos; a.block_tables = g->block_tables;
+    a.rope_cos = g->rope_cos; a.rope_sin = g->rope_sin;
+    a.dtype = g->dtype; a.B = g->B; a.T = g->T; a.n_heads = g->n_heads; a.max_pages = g->max_pages; a.layer = g->layer;
+    a.rope_len = g->rope_len; a.rot_dim = g->rot_dim; a.rope_layout = g->rope_layout; a.err = error_flag;
+    return nitro::launch_kv8_append(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+}
+
+size_t nr_paged_attention_kv8_workspace_size(int32_t B, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                             int32_t max_pages) {
+    if (B <= 0 || B > 1024 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 16 ||
+        n_heads > (1 << 16) || (head_dim != 64 && head_dim != 128) || max_pages <= 0 || max_pages > (1 << 26))
+        return 0;
+    return nitro::kv8_decode_workspace_bytes(B, n_heads, n_kv_heads, head_dim, max_pages);
+}
+
+int nr_paged_attention_decode_kv8(const void* q, int32_t dtype, const nr_kv8_pool* pool, int32_t layer,
+                                  const int32_t* block_tables, int32_t max_pages, const int32_t* ctx_lens, int32_t B,
+                                  int32_t n_heads, void* out, void* workspace, int32_t* error_flag, void* stream) {
+    nitro::Kv8DecodeArgs a;
+    if (!q || !block_tables || !ctx_lens || !out || !workspace || !valid_dtype(dtype)) return NR_ERR_INVALID;
+    if (!read_kv8_pool(pool, layer, &a.pool) || !aligned16(q) || !aligned16(out) || !aligned16(workspace)) return NR_ERR_INVALID;
+    if (!nr_paged_attention_kv8_workspace_size(B, n_heads, pool->n_kv_heads, pool->head_dim, max_pages)) return NR_ERR_INVALID;
+    a.q = q; a.out = out; a.block_tables = block_tables; a.ctx_lens = ctx_lens; a.workspace = workspace;
+    a.dtype = dtype; a.layer = layer; a.max_pages = max_pages; a.B = B; a.n_heads = n_heads; a.err = error_flag;
+    return nitro::launch_kv8_decode(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+}
+
+int nr_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                        int64_t v_stride, void* out, int64_t out_stride, int32_t dtype, const int32_t* cu_q,
+                        const int32_t* cu_k, int32_t B, int32_t Tq, int32_t Tk, int32_t n_heads, int32_t n_kv_heads,
+                        int32_t head_dim, int32_t* error_flag, void* stream) {
+    if (dtype != NR_DTYPE_BF16 && dtype != NR_DTYPE_F16) return NR_ERR_INVALID;
+    if (!cu_q || B <= 0 || B > 1024 || Tq <= 0 || Tk <= 0 || (!cu_k && Tq != Tk)) return NR_ERR_INVALID;
+    if (n_heads <= 0 || n_heads > (1 << 15) || n_kv_heads <= 0 || n_heads % n_kv_heads) return NR_ERR_INVALID;
+    if (head_dim != 64 && head_dim != 128) return NR_ERR_INVALID;
+    const int64_t qw = (int64_t)n_heads * head_dim, kw = (int64_t)n_kv_heads * head_dim;
+    if (!valid_rows(q, q_stride, qw, dtype) || !valid_rows(out, out_stride, qw, dtype) ||
+        !valid_rows(k, k_stride, kw, dtype) || !valid_rows(v, v_stride, kw, dtype))
+        return NR_ERR_INVALID;
+    nitro::PromptAttnArgs a;
+    a.q = q; a.k = k; a.v = v; a.out = out; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+    a.out_stride = out_stride; a.cu_q = cu_q; a.cu_k = cu_k; a.dtype = dtype; a.B = B; a.Tq = Tq; a.Tk = Tk;
+    a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.head_dim = head_dim; a.err = error_flag;
+    return nitro::launch_prompt_attention(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+}
+
+int nr_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int32_t M, int32_t V,
+                      const int32_t* targets, int32_t top_k, float* target_logprob, float* entropy, float* top_logprob,
+                      int32_t* top_ids, void* stream) {
+    if (!logits || !valid_dtype(dtype) || M <= 0 || V <= 0 || row_stride < V) return NR_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(logits) % nitro::dtype_bytes(dtype)) return NR_ERR_INVALID;
+    if (top_k < 0 || top_k > NR_LOGPROBS_MAX_TOP || top_k > V || !targets != !target_logprob) return NR_ERR_INVALID;
+    if (top_k ? !top_logprob || !top_ids : top_logprob || top_ids) return NR_ERR_INVALID;
+    if (!target_logprob && !entropy && !top_k) return NR_ERR_INVALID;
+    nitro::LogprobArgs a;
+    a.logits = logits; a.dtype = dtype; a.row_stride = row_stride; a.M = M; a.V = V; a.top_k = top_k;
+    a.targets = targets; a.target_logprob = target_logprob; a.entropy = entropy; a.top_logprob = top_logprob;
+    a.top_ids = top_ids;
+    return nitro::launch_token_logprobs(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
 }
 
 size_t nr_q8_quantized_size(int64_t n) { return nitro::q8_quantized_bytes(n); }

@@ -1,0 +1,194 @@
+"""nr_paged_attention_decode_kv8 against 64-bit attention over the same codes."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from kv8_util import DTYPES, PAGE, Pool, assert_within, attend, bound, decode, i32, tables  # noqa: E402
+from nitrorag_b200._lib import lib  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+# weights enter the products as fp16 (16-bit types) or as two fp16 halves (fp32)
+P_ROUND = {"f32": 2.0 ** -20, "bf16": 2.0 ** -11, "f16": 2.0 ** -11}
+
+
+@pytest.fixture(autouse=True)
+def need_gpu():
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required for gpu tests")
+
+
+def reference(pool, q, table, ctx, layer, pages_ok=None):
+    """(out, sum p|v|, size) in 64 bits; page ids outside the pool are absent tokens."""
+    B, H, hd = q.shape
+    n_pages, _, KV, _ = pool.shape4
+    out, pv, size = (torch.zeros(s, dtype=torch.float64, device="cuda") for s in ((B, H, hd), (B, H, hd), (B, H)))
+    for b in range(B):
+        n = min(max(int(ctx[b]), 0), table.shape[1] * PAGE)
+        ids = table[b, :(n + PAGE - 1) // PAGE].long()
+        there = (ids >= 0) & (ids < n_pages)
+        here = there.repeat_interleave(PAGE)[:n]
+        ids = torch.where(there, ids, torch.zeros_like(ids))
+        for j in range(KV):
+            kk, vv = (getattr(pool, x)[ids, layer, j].view(torch.float8_e4m3fn).double()
+                      * getattr(pool, x + "_scale")[ids, layer, j].double()[:, None, None] for x in "kv")
+            kk, vv = (t.reshape(-1, hd)[:n][here] for t in (kk, vv))
+            g = H // KV
+            seen = torch.ones((g, len(kk)), dtype=torch.bool, device="cuda")
+            r = attend(q[b, j * g:(j + 1) * g].double(), kk, vv, seen)
+            out[b, j * g:(j + 1) * g], pv[b, j * g:(j + 1) * g], size[b, j * g:(j + 1) * g] = r
+    return out, pv, size
+
+
+def check(pool, q, table, ctx, layer, dtype, flag=0, **kw):
+    err = i32([0])
+    got = decode(pool, q, table, ctx, layer=layer, err=err, **kw)
+    want, pv, size = reference(pool, q, table, ctx, layer)
+    assert int(err) == flag
+    assert_within(got, want, bound(dtype, want, pv, size, P_ROUND[dtype]), "decode")
+    return got
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,H,KV", [(64, 12, 12), (128, 4, 4), (64, 8, 2), (128, 32, 4), (64, 7, 1), (128, 9, 3),
+                                     (64, 16, 1), (128, 24, 2), (64, 1, 1)])
+def test_decode(dtype, hd, H, KV):
+    """Lengths of zero and one, page borders and long ones; a middle layer; table entries behind a
+    context hold ids outside the pool; NaN codes and NaN scales behind the last token and in pages not used."""
+    rng = np.random.default_rng(hd + H)
+    ctx = [1, 0, 15, 16, 17, 128, 129, 300, 1030, 0, 64]
+    counts = [(n + PAGE - 1) // PAGE for n in ctx]
+    P = sum(counts) + 5
+    pool = Pool(P, 3, KV, hd, seed=H)
+    table = tables(rng, counts, P)
+    used = torch.zeros(P, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(ctx):
+        for i in range(counts[b]):
+            used[int(table[b, i])] = True
+        if n % PAGE:
+            page = int(table[b, counts[b] - 1])
+            for t in (pool.k, pool.v):
+                t[page, :, :, n % PAGE:] = 0x7f  # NaN
+    for t in (pool.k, pool.v):
+        t[~used] = 0x7f
+    pool.k_scale[~used] = float("nan")
+    q = torch.randn((len(ctx), H, hd), device="cuda", generator=torch.Generator(device="cuda").manual_seed(H)).to(DTYPES[dtype][1])
+    got = check(pool, q, table, i32(ctx), 1, dtype)
+    assert torch.equal(got[1], torch.zeros_like(got[1]))
+    assert torch.equal(got, decode(pool, q, table, i32(ctx), layer=1))  # a fixed order of sums
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,H,KV,hd,n", [(1, 8, 8, 64, 5000), (2, 8, 1, 128, 20011), (1, 32, 8, 128, 40000), (70, 2, 2, 64, 333)])
+def test_long_and_wide(dtype, B, H, KV, hd, n):
+    rng = np.random.default_rng(n)
+    ctx = [max(n - 7 * b, b) for b in range(B)]
+    counts = [(c + PAGE - 1) // PAGE for c in ctx]
+    pool = Pool(sum(counts), 1, KV, hd, seed=3)
+    table = tables(rng, counts, sum(counts))
+    q = torch.randn((B, H, hd), device="cuda").to(DTYPES[dtype][1])
+    check(pool, q, table, i32(ctx), 0, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_peaked_and_shifted_scores(dtype):
+    """Scores that rise along the context (the running maximum moves in every page), one token that takes
+    all the weight, and blocks whose scales differ by many powers of two."""
+    hd, H, KV = 64, 4, 2
+    n = 400
+    pool = Pool(25, 1, KV, hd, seed=1)
+    table = i32([list(range(25))] * 3)
+    order = torch.arange(25, device="cuda").float()
+    pool.k_scale *= torch.exp2(order - 12)[:, None, None].clamp(2.0 ** -6, 2.0 ** 3)
+    pool.v_scale *= torch.exp2(3 * (order % 7) - 9)[:, None, None]
+    q = torch.randn((3, H, hd), device="cuda").to(DTYPES[dtype][1])
+    q[1] *= 30
+    q[2] *= 1e-3
+    check(pool, q, table, i32([n, n - 3, n]), 0, dtype)
+
+
+def test_small_values_keep_their_precision():
+    """Values of 2^-40 and queries of 2^-30 and 2^40: nothing passes through a fixed-range 16-bit format."""
+    hd, H, KV = 128, 2, 1
+    for vs, qs, ks in ((2.0 ** -40, 1.0, 1.0), (2.0 ** 60, 2.0 ** -30, 2.0 ** 30), (1.0, 2.0 ** 40, 2.0 ** -40)):
+        pool = Pool(8, 1, KV, hd, seed=2)
+        pool.v_scale *= vs
+        pool.k_scale *= ks
+        table = i32([list(range(8))])
+        q = torch.randn((1, H, hd), device="cuda") * qs
+        check(pool, q, table, i32([121]), 0, "f32")
+
+
+def test_nan_block_reaches_only_its_readers():
+    hd, H, KV = 64, 2, 2
+    pool = Pool(8, 1, KV, hd, seed=4)
+    pool.k_scale[5, 0, 1] = float("nan")
+    table = i32([[0, 1, 2, 3], [4, 5, 6, 7]])
+    q = torch.randn((2, H, hd), device="cuda")
+    got = decode(pool, q, table, i32([64, 60]))
+    assert bool(got[1, 1].isnan().all()) and bool(got[0].isfinite().all()) and bool(got[1, 0].isfinite().all())
+
+
+@pytest.mark.parametrize("B", [3, 64])
+def test_bad_lengths_and_pages(B):
+    """Too long, negative, and bad page ids: flagged, clamped or absent, the other rows unchanged."""
+    hd, H, KV, width = 64, 4, 2, 8
+    rng = np.random.default_rng(B)
+    pool = Pool(B * width, 1, KV, hd, seed=6)
+    table = tables(rng, [width] * B, B * width)
+    ctx = rng.integers(1, width * PAGE + 1, B).tolist()
+    q = torch.randn((B, H, hd), device="cuda")
+    for b, n in ((0, width * PAGE + 1), (1, -5), (2, 2 ** 31 - 1)):
+        c = list(ctx)
+        c[b] = n
+        check(pool, q, table, i32(c), 0, "f32", flag=2)
+    for page in (-1, B * width, 2 ** 31 - 1):
+        t, c = table.clone(), list(ctx)
+        c[1] = width * PAGE - 3
+        t[1, 2] = page
+        check(pool, q, t, i32(c), 0, "f32", flag=2)
+    t = table.clone()
+    t[0] = -1
+    c = list(ctx)
+    c[0] = 100
+    got = check(pool, q, t, i32(c), 0, "f32", flag=2)
+    assert torch.equal(got[0], torch.zeros_like(got[0]))
+
+
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 codes: pages at its far end."""
+    hd, H, KV, layers = 128, 8, 8, 4
+    P = (1 << 32) // (layers * KV * PAGE * hd) + 20
+    pool = Pool.__new__(Pool)
+    pool.shape4 = (P, layers, KV, hd)
+    for n in "kv":
+        setattr(pool, n, torch.zeros((P, layers, KV, PAGE, hd), dtype=torch.uint8, device="cuda"))
+        setattr(pool, n + "_scale", torch.ones((P, layers, KV), device="cuda"))
+    small = Pool(16, layers, KV, hd, seed=8)
+    for n in ("k", "v", "k_scale", "v_scale"):
+        getattr(pool, n)[-16:] = getattr(small, n)
+    q = torch.randn((1, H, hd), device="cuda")
+    far = decode(pool, q, i32([list(range(P - 16, P))]), i32([250]), layer=3)
+    assert torch.equal(far, decode(small, q, i32([list(range(16))]), i32([250]), layer=3))
+
+
+def test_workspace_is_left_ready_and_can_be_shared_in_order():
+    """Calls of different shapes one after another over one workspace; a captured graph replayed between them."""
+    hd = 64
+    size = max(lib().nr_paged_attention_kv8_workspace_size(b, h, kv, hd, w) for b, h, kv, w in ((1, 8, 8, 600), (40, 4, 1, 20)))
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(0)
+    a = Pool(600, 1, 8, hd, seed=1), tables(rng, [600], 600), i32([9590]), torch.randn((1, 8, hd), device="cuda")
+    b = Pool(800, 1, 1, hd, seed=2), tables(rng, [20] * 40, 800), i32(rng.integers(0, 321, 40).tolist()), torch.randn((40, 4, hd), device="cuda")
+    want = [decode(p, q, t, c) for p, t, c, q in (a, b)]
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(a[3])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        decode(a[0], a[3], a[1], a[2], out=out, ws=ws)
+    for _ in range(3):
+        assert torch.equal(decode(b[0], b[3], b[1], b[2], ws=ws), want[1])
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want[0])
+        assert torch.equal(decode(a[0], a[3], a[1], a[2], ws=ws), want[0])
