@@ -1,7 +1,32 @@
 // Decode attention over e4m3 pages (nr_paged_attention_decode_kv8).
 //
-// One CTA per (sequence, head): each warp takes every fourth page with its own running
-// maximum, sum and output (lane l holds dims l, l + 32, ...), joined through shared memory.
+// One query row per sequence: every cached byte is used once for each of the query heads
+// that share it, so the kernel is bound by reading the pages.  A page's 16 tokens are the
+// M = 16 rows of mma.m16n8k16 and up to 8 query heads of a group its N = 8 columns:
+//
+//   S^T[token][head] = K[token][dim] Q^T[dim][head]
+//   O^T[dim][head]  += V^T[dim][token] W[token][head]
+//
+// e4m3 values are exact in fp16, so K and V enter the products unrounded (one conversion
+// for two values).  The order of the summed dims and tokens is free, which lets each lane
+// load 16 contiguous bytes of its rows straight from global memory into fragment order: no
+// shared memory, and no barrier between the warps until the end.
+//
+// fp16 has few exponent bits, so both small operands are scaled by powers of two (exact):
+// a query row to a largest value of 2^7, and the weights W = p * v_scale * gain with a gain
+// per head that puts the largest weight so far near 2^7, so that what matters in the sum
+// is never below fp16's normal range whatever the blocks' scales are.  p = exp2(s - m) goes by a
+// running maximum that is only moved when a score passes it by 8 (a weight of at most 2^8
+// costs no precision), so most pages need no exchange between lanes.  16-bit inputs round
+// a weight once to fp16 (2^-11, under the output's own rounding); fp32 inputs carry query
+// and weights as two fp16 halves (22 bits) and take each product twice.
+//
+// Work: the pages of all (sequence, kv head) items are cut into units of about equal
+// length, one CTA each, its four warps taking every fourth page.  The cut goes by the
+// lengths on the device, so a ragged batch and a table much wider than its contexts cost
+// nothing.  An item of one unit is finished by its CTA; otherwise the partial results go
+// to the workspace and the item's last CTA joins them in order (the result does not
+// depend on which CTA that is).
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
@@ -16,81 +41,463 @@ namespace nitro {
 namespace {
 
 constexpr int kWarps = 4;
+// Units to cut a batch into: three CTAs are resident on each of 148 SMs.
+constexpr int kUnits = 3 * 148;
+constexpr int kMinPages = 8;            // of a unit: two for each warp
+// Items whose partial results can be counted; more items than that fill the device uncut.
+constexpr int kCounters = 16384;
+constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float e4m3_f32(uint8_t c) {
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kWarps * 32) kv8_decode_kernel(Kv8DecodeArgs a) {
-    constexpr int D = HD / 32;
-    __shared__ float s_m[kWarps], s_l[kWarps], s_o[kWarps][HD];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int h = blockIdx.x, b = blockIdx.y;
+// Two e4m3 codes (low and high byte) as fp16, exact.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint16_t c) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(c));
+    return d;
+}
+__device__ __forceinline__ void word_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    lo = e4m3x2_f16x2((uint16_t)w);
+    hi = e4m3x2_f16x2((uint16_t)(w >> 16));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+// What is left of two values after their rounding to fp16 in h.
+__device__ __forceinline__ uint32_t pack_f16_rest(float lo, float hi, uint32_t h) {
+    const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    return pack_f16(lo - r.x, hi - r.y);
+}
+
+__device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transpose of an 8x8 matrix of 16-bit values held one row to four lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load8(const uint8_t* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+
+// 2^(7 - exponent of x), within the normal range; 1 for zero, infinities and NaN.
+__device__ __forceinline__ float gain_of(float x) {
+    const int e = (int)((__float_as_uint(x) >> 23) & 0xff);
+    if (!(x > 0.0f) || e == 255) return 1.0f;
+    return __uint_as_float((uint32_t)min(max(261 - e, 2), 252) << 23);
+}
+
+// A lane's part of one page: with g = lane / 4, c = lane % 4, bytes 16c.. of each 64 of K's
+// rows g and g + 8, and bytes g*HD/8.. of V's rows 2c, 2c+1, 2c+8, 2c+9.
+template <int HD>
+struct PageRegs {
+    uint32_t k[2][HD / 64][4];
+    uint32_t v[4][HD / 32];
+    __device__ __forceinline__ void load(const uint8_t* kt, const uint8_t* vt, int g, int c) {
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int j = 0; j < HD / 64; j++) {
+                const uint4 u = load16(kt + (g + 8 * r) * HD + 64 * j + 16 * c);
+                k[r][j][0] = u.x; k[r][j][1] = u.y; k[r][j][2] = u.z; k[r][j][3] = u.w;
+            }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint8_t* p = vt + (2 * c + (t & 1) + 8 * (t >> 1)) * HD + g * (HD / 8);
+            if constexpr (HD == 128) {
+                const uint4 u = load16(p);
+                v[t][0] = u.x; v[t][1] = u.y; v[t][2] = u.z; v[t][3] = u.w;
+            } else {
+                const uint2 u = load8(p);
+                v[t][0] = u.x; v[t][1] = u.y;
+            }
+        }
+    }
+};
+
+// Running state of one warp: NT tiles of 8 heads; a lane's columns are heads 2c, 2c + 1 of
+// each, its output rows dims g*HD/8 .. + HD/8 - 1.
+template <int HD, int NT, bool SPLIT>
+struct WarpState {
+    uint32_t q[SPLIT ? 2 : 1][NT][HD / 64][8];
+    float o[NT][HD / 16][4];
+    float m[NT][2], l[NT][2], wmax[NT][2], gain[NT][2], factor[NT][2];
+
+    __device__ __forceinline__ void page(const PageRegs<HD>& r, float ks, float vs, int valid, int g, int c) {
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[n][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint32_t a0, a1, a2, a3;
+                word_f16(r.k[0][j][w], a0, a2);
+                word_f16(r.k[1][j][w], a1, a3);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    mma_f16(s[n], a0, a1, a2, a3, q[0][n][j][2 * w], q[0][n][j][2 * w + 1]);
+                    if constexpr (SPLIT) mma_f16(s[n], a0, a1, a2, a3, q[1][n][j][2 * w], q[1][n][j][2 * w + 1]);
+                }
+            }
+        bool moves = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[n][i] *= ks * factor[n][i & 1];
+            if (valid < kPage) {
+                if (g >= valid) s[n][0] = s[n][1] = -INFINITY;
+                if (g + 8 >= valid) s[n][2] = s[n][3] = -INFINITY;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                moves |= fmaxf(s[n][h], s[n][2 + h]) > m[n][h] + 8.0f || vs * gain[n][h] > 128.0f;
+        }
+        if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float t = fmaxf(s[n][h], s[n][2 + h]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, x));
+                    const float mn = fmaxf(m[n][h], t);
+                    const float corr = m[n][h] == -INFINITY ? 0.0f : exp2_fast(m[n][h] - mn);
+                    const float now = t == -INFINITY ? 0.0f : exp2_fast(t - mn) * vs;
+                    wmax[n][h] = fmaxf(wmax[n][h] * corr, now);
+                    const float next = gain_of(wmax[n][h]);
+                    const float f = corr * next * (1.0f / gain[n][h]);
+                    l[n][h] *= corr;
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++) {
+                        o[n][i][h] *= f;
+                        o[n][i][2 + h] *= f;
+                    }
+                    m[n][h] = mn;
+                    gain[n][h] = next;
+                }
+        }
+        uint32_t b[SPLIT ? 2 : 1][NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float p = exp2_fast(s[n][i] - m[n][i & 1]);
+                l[n][i & 1] += p;
+                w[i] = p * (vs * gain[n][i & 1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t hi = pack_f16(w[2 * i], w[2 * i + 1]);
+                b[0][n][i] = transpose8(hi);
+                if constexpr (SPLIT) b[1][n][i] = transpose8(pack_f16_rest(w[2 * i], w[2 * i + 1], hi));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) {
+            // bytes 2i, 2i + 1 of the lane's 4 rows: adjacent tokens' values of a dim side by side
+            const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
+            uint32_t v0 = r.v[0][i / 2], v1 = r.v[1][i / 2], v2 = r.v[2][i / 2], v3 = r.v[3][i / 2];
+            if (valid < kPage) {  // what lies behind the last token may be NaN
+                if (2 * c >= valid) v0 = 0;
+                if (2 * c + 1 >= valid) v1 = 0;
+                if (2 * c + 8 >= valid) v2 = 0;
+                if (2 * c + 9 >= valid) v3 = 0;
+            }
+            uint32_t a0, a1, a2, a3;
+            word_f16(__byte_perm(v0, v1, sel), a0, a1);
+            word_f16(__byte_perm(v2, v3, sel), a2, a3);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                mma_f16(o[n][i], a0, a1, a2, a3, b[0][n][0], b[0][n][1]);
+                if constexpr (SPLIT) mma_f16(o[n][i], a0, a1, a2, a3, b[1][n][0], b[1][n][1]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ int context_of(const Kv8DecodeArgs& a, int b, bool& bad) {
+    const int64_t n = a.ctx_lens[b], cap = (int64_t)a.max_pages * kPage;
+    bad = n < 0 || n > cap;
+    return (int)((n < 0 ? 0 : n > cap ? cap : n) + kPage - 1) / kPage;
+}
+
+// exp2(m - top), for a part without tokens 0 (or its NaN).
+__device__ __forceinline__ float part_weight(float m, float top, float l) {
+    return m == -INFINITY ? (l != l ? l : 0.0f) : exp2_fast(m - top);
+}
+
+// Floats of a unit's partial result: group rows of HD values, then the group's maxima and
+// sums, a whole number of 16-byte pieces.
+__host__ __device__ __forceinline__ int64_t partial_floats(int group, int head_dim) {
+    return (int64_t)group * head_dim + (2 * group + 3) / 4 * 4;
+}
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(kWarps * 32, HD * NT == 256 ? 2 : 3) kv8_decode_kernel(Kv8DecodeArgs a, float* partial, int* counters) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int HEADS = 8 * NT, LD = HD + 4;
+    __shared__ __align__(16) float s_o[kWarps][HEADS][LD], s_m[kWarps][HEADS], s_l[kWarps][HEADS];
+    __shared__ int s_last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int nkv = a.pool.n_kv_heads, group = a.n_heads / nkv;
     grid_dependency_wait();
     grid_dependents_launch();
-    int ctx = a.ctx_lens[b];
-    if (ctx < 0 || ctx > (int64_t)a.max_pages * kPage) {
-        if (threadIdx.x == 0) flag_error(a.err, kErrBadContext);
-        ctx = ctx < 0 ? 0 : a.max_pages * kPage;
+
+    // the cut: all pages over kUnits, then the sequence this unit belongs to
+    int64_t total = 0;
+    bool any_bad = false;
+    for (int i = lane; i < a.B; i += 32) {
+        bool bad;
+        total += context_of(a, i, bad);
+        any_bad |= bad;
     }
-    const int nkv = a.pool.n_kv_heads, kvh = h / (a.n_heads / nkv);
-    const T* q = (const T*)a.q + ((int64_t)b * a.n_heads + h) * HD;
-    float qv[D], o[D], m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D; i++) {
-        qv[i] = to_f32(q[lane + 32 * i]) * rsqrtf((float)HD);
-        o[i] = 0.0f;
-    }
-    for (int pg = warp; pg * kPage < ctx; pg += kWarps) {
-        const int page = a.block_tables[(int64_t)b * a.max_pages + pg];
-        if (page < 0 || page >= a.pool.n_pages) {
-            if (lane == 0) flag_error(a.err, kErrBadContext);
-            continue;
+    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    if (blockIdx.x == 0 && any_bad) flag_error(a.err, kErrBadContext);
+    const int64_t per = (total * nkv + kUnits - 1) / kUnits;
+    const int chunk = (int64_t)a.B * nkv > kCounters ? INT32_MAX : (int)max((int64_t)kMinPages, min(per, (int64_t)INT32_MAX));
+    const int unit = blockIdx.x;
+    int b = -1, pages = 0, units = 0, at = 0;  // at: first unit of sequence b
+    for (int i0 = 0, before = 0; i0 < a.B && b < 0; i0 += 32) {
+        const int i = i0 + lane;
+        bool bad;
+        const int n = i < a.B ? context_of(a, i, bad) : 0;
+        const int u = i < a.B ? max(1, (int)(((int64_t)n + chunk - 1) / chunk)) : 0;  // an empty row is written too
+        int sum = u;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, x);
+            if (lane >= x) sum += y;
         }
-        const int64_t block = ((int64_t)page * a.pool.n_layers + a.layer) * nkv + kvh;
-        const float ks = a.pool.k_scale[block], vs = a.pool.v_scale[block];
-        for (int r = 0; r < min(kPage, ctx - pg * kPage); r++) {
-            float x = 0.0f;
+        const uint32_t past = __ballot_sync(0xffffffffu, (int64_t)(before + sum) * nkv > unit);
+        if (past) {
+            const int src = __ffs(past) - 1;
+            b = i0 + src;
+            pages = __shfl_sync(0xffffffffu, n, src);
+            units = __shfl_sync(0xffffffffu, u, src);
+            at = before + __shfl_sync(0xffffffffu, sum - u, src);
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (b < 0) return;
+    const int kvh = (unit - at * nkv) % nkv, part = (unit - at * nkv) / nkv;
+    const int each = (pages + units - 1) / units;
+    const int pg0 = part * each, pg1 = min(pages, pg0 + each);
+    const int ctx = min(max(a.ctx_lens[b], 0), pages * kPage);
+
+    WarpState<HD, NT, SPLIT> st;
 #pragma unroll
-            for (int i = 0; i < D; i++) x += qv[i] * e4m3_f32(a.pool.k[(block * kPage + r) * HD + lane + 32 * i]);
-            x = warp_sum(x) * ks;
-            const float mn = fmaxf(m, x);
-            const float c = m == -INFINITY ? 0.0f : expf(m - mn), p = x == -INFINITY ? 0.0f : expf(x - mn);
-            m = mn;
-            l = l * c + p;
+    for (int n = 0; n < NT; n++) {
+        const int head = 8 * n + g;
+        float x[HD / 64][16], top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D; i++)
-                o[i] = o[i] * c + p * vs * e4m3_f32(a.pool.v[(block * kPage + r) * HD + lane + 32 * i]);
+        for (int j = 0; j < HD / 64; j++)
+            if (head < group) {
+                const T* p = (const T*)a.q + ((int64_t)b * a.n_heads + kvh * group + head) * HD + 64 * j + 16 * c;
+#pragma unroll
+                for (int v = 0; v < (int)sizeof(T); v++) {
+                    const uint4 u = reinterpret_cast<const uint4*>(p)[v];
+                    const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+                    for (int i = 0; i < 16 / (int)sizeof(T); i++) x[j][v * (16 / (int)sizeof(T)) + i] = to_f32(t[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) x[j][i] = 0.0f;
+            }
+#pragma unroll
+        for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, fabsf(x[j][i]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float up = std::is_same<T, __half>::value ? 1.0f : gain_of(top);
+#pragma unroll
+        for (int j = 0; j < HD / 64; j++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float x0 = x[j][2 * i] * up, x1 = x[j][2 * i + 1] * up;
+                st.q[0][n][j][i] = pack_f16(x0, x1);
+                if constexpr (SPLIT) st.q[1][n][j][i] = pack_f16_rest(x0, x1, st.q[0][n][j][i]);
+            }
+        const float down = (1.0f / up) * (kLog2e * rsqrtf((float)HD));
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            st.factor[n][h] = __shfl_sync(0xffffffffu, down, (2 * c + h) * 4);
+            st.m[n][h] = -INFINITY;
+            st.l[n][h] = st.wmax[n][h] = 0.0f;
+            st.gain[n][h] = 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) st.o[n][i][k] = 0.0f;
+    }
+
+    // this warp's pages, 32 at a time: lane i looks up the i-th one's block and scales
+    const int mine = pg1 - pg0 > warp ? (pg1 - pg0 - warp + kWarps - 1) / kWarps : 0;
+    for (int base = 0; base < mine; base += 32) {
+        const int count = min(32, mine - base);
+        int64_t block = -1;
+        float ks = 0.0f, vs = 0.0f;
+        if (lane < count) {
+            const int pg = pg0 + warp + kWarps * (base + lane);
+            const int id = a.block_tables[(int64_t)b * a.max_pages + pg];
+            if (id >= 0 && id < a.pool.n_pages) {
+                block = ((int64_t)id * a.pool.n_layers + a.layer) * nkv + kvh;
+                ks = a.pool.k_scale[block];
+                vs = a.pool.v_scale[block];
+            } else {
+                flag_error(a.err, kErrBadContext);
+            }
+        }
+        PageRegs<HD> r[2];
+        auto fetch = [&](PageRegs<HD>& x, int i) {
+            const int64_t blk = __shfl_sync(0xffffffffu, block, i);
+            if (blk >= 0) x.load(a.pool.k + blk * (kPage * HD), a.pool.v + blk * (kPage * HD), g, c);
+        };
+        auto use = [&](const PageRegs<HD>& x, int i) {
+            const int64_t blk = __shfl_sync(0xffffffffu, block, i);
+            const float kk = __shfl_sync(0xffffffffu, ks, i), vv = __shfl_sync(0xffffffffu, vs, i);
+            const int left = ctx - (pg0 + warp + kWarps * (base + i)) * kPage;
+            if (blk >= 0) st.page(x, kk, vv, left, g, c);
+        };
+        fetch(r[0], 0);
+        for (int i = 0; i < count; i += 2) {
+            if (i + 1 < count) fetch(r[1], i + 1);
+            use(r[0], i);
+            if (i + 1 < count) {
+                if (i + 2 < count) fetch(r[0], i + 2);
+                use(r[1], i + 1);
+            }
         }
     }
-    if (lane == 0) s_m[warp] = m, s_l[warp] = l;
+
+    // join the warps
 #pragma unroll
-    for (int i = 0; i < D; i++) s_o[warp][lane + 32 * i] = o[i];
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float l = st.l[n][h];
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+            const int head = 8 * n + 2 * c + h;
+            if (g == 0) s_m[warp][head] = st.m[n][h], s_l[warp][head] = l;
+            const float down = 1.0f / st.gain[n][h];
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) {
+                float2 v = make_float2(st.o[n][i][h] * down, st.o[n][i][2 + h] * down);
+                *reinterpret_cast<float2*>(&s_o[warp][head][g * (HD / 8) + 2 * i]) = v;
+            }
+        }
     __syncthreads();
-    float mm = -INFINITY;
-    for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, s_m[w]);
-    for (int d = threadIdx.x; d < HD; d += blockDim.x) {
-        float sum = 0.0f, acc = 0.0f;
+    const int64_t rec = partial_floats(group, HD);
+    float* mine_out = partial + (int64_t)unit * rec;
+    T* out = (T*)a.out + ((int64_t)b * a.n_heads + kvh * group) * HD;
+    for (int e = threadIdx.x * 4; e < group * HD; e += blockDim.x * 4) {
+        const int head = e / HD, d = e % HD;
+        float top = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) top = fmaxf(top, s_m[w][head]);
+#pragma unroll
         for (int w = 0; w < kWarps; w++) {
-            const float c = s_m[w] == -INFINITY ? (s_l[w] != s_l[w] ? s_l[w] : 0.0f) : expf(s_m[w] - mm);
-            sum += c * s_l[w];
-            acc += c * s_o[w][d];
+            const float f = part_weight(s_m[w][head], top, s_l[w][head]);
+            l += f * s_l[w][head];
+            const float4 v = *reinterpret_cast<const float4*>(&s_o[w][head][d]);
+            acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
         }
-        ((T*)a.out)[((int64_t)b * a.n_heads + h) * HD + d] = from_f32<T>(sum == 0.0f ? 0.0f : acc / sum);
+        if (units == 1) {
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[e + i] = from_f32<T>(acc[i] * inv);
+        } else {
+            *reinterpret_cast<float4*>(mine_out + e) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            if (d == 0) mine_out[group * HD + head] = top, mine_out[group * HD + group + head] = l;
+        }
     }
+    if (units == 1) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int* n = counters + b * nkv + kvh;
+        const int before = atomicAdd(n, 1);
+        s_last = before == units - 1;
+        if (s_last) *n = 0;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    const float* first = partial + ((int64_t)at * nkv + kvh) * rec;
+    const int64_t step = (int64_t)nkv * rec;
+    for (int e = threadIdx.x * 4; e < group * HD; e += blockDim.x * 4) {
+        const int head = e / HD;
+        float top = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int u = 0; u < units; u++) top = fmaxf(top, __ldcg(first + u * step + group * HD + head));
+#pragma unroll 4
+        for (int u = 0; u < units; u++) {
+            const float* p = first + u * step;
+            const float pl = __ldcg(p + group * HD + group + head);
+            const float f = part_weight(__ldcg(p + group * HD + head), top, pl);
+            l += f * pl;
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + e));
+            acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[e + i] = from_f32<T>(acc[i] * inv);
+    }
+}
+
+int64_t most_units(int B, int n_kv_heads) { return (int64_t)B * n_kv_heads + kUnits; }
+
+template <typename T, int HD>
+cudaError_t launch_hd(const Kv8DecodeArgs& a, cudaStream_t s) {
+    int* counters = (int*)a.workspace;
+    float* partial = (float*)((char*)a.workspace + kCounters * sizeof(int));
+    const dim3 grid((unsigned)most_units(a.B, a.pool.n_kv_heads));
+    if (a.n_heads / a.pool.n_kv_heads <= 8)
+        return launch_ex(kv8_decode_kernel<T, HD, 1>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters);
+    return launch_ex(kv8_decode_kernel<T, HD, 2>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters);
 }
 
 template <typename T>
 cudaError_t launch_t(const Kv8DecodeArgs& a, cudaStream_t s) {
-    const dim3 grid(a.n_heads, a.B);
-    if (a.pool.head_dim == 64) return launch_ex(kv8_decode_kernel<T, 64>, grid, dim3(kWarps * 32), 0, s, 1, a);
-    return launch_ex(kv8_decode_kernel<T, 128>, grid, dim3(kWarps * 32), 0, s, 1, a);
+    return a.pool.head_dim == 64 ? launch_hd<T, 64>(a, s) : launch_hd<T, 128>(a, s);
 }
 
 }  // namespace
 
-size_t kv8_decode_workspace_bytes(int, int, int, int, int) { return 256; }
+size_t kv8_decode_workspace_bytes(int B, int n_heads, int n_kv_heads, int head_dim, int) {
+    const size_t rec = partial_floats(n_heads / n_kv_heads, head_dim) * sizeof(float);
+    const size_t n = (int64_t)B * n_kv_heads > kCounters ? 0 : (size_t)most_units(B, n_kv_heads) * rec;
+    return kCounters * sizeof(int) + (n + 255) / 256 * 256;
+}
 
 cudaError_t launch_kv8_decode(const Kv8DecodeArgs& a, cudaStream_t s) {
     count_launch();
