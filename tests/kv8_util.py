@@ -136,13 +136,18 @@ def attend(q, k, v, seen):
     return p @ v, p @ v.abs(), size
 
 
-def bound(dtype, out, pv, size, p_round):
+def bound(dtype, out, pv, size, p_round, small=0.0):
     """|error| of an attention output: scores carry 2^-20 of |q|max sum|k| / sqrt(hd) (22-bit products of
     the split query, fp32 sums of up to 128 terms, the scale and log2 e factors), which moves a weight by
     that much relatively, twice with the normalisation; exp2 and sums 2^-17; weights rounded to the
-    products' type (p_round); the output rounded once to its own."""
+    products' type (p_round); the output rounded once to its own.  fp16 values below 2^-14 are 2^-24
+    apart, so there half a step is 2^-25 whatever the value: for the output, and for each weight
+    (`small`: sum |v| over the keys seen, where weights enter a product as fp16 relative to a maximum near 1)."""
     rel = 2 * 2.0 ** -20 * size[..., None] + 2.0 ** -17 + p_round
-    return rel * pv + HALF[dtype] * out.abs() + 1e-30
+    own = HALF[dtype] * out.abs()
+    if dtype == "f16":
+        own = own.clamp(min=2.0 ** -25) + 2.0 ** -25 * small
+    return rel * pv + own + 1e-30
 
 
 def assert_within(got, want, tol, what):

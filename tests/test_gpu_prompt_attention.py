@@ -31,7 +31,7 @@ def call(q, k, v, out, cu_q, cu_k, B, H, KV, hd, err=None, Tq=None, Tk=None, exp
 def reference(q, k, v, lens_q, lens_k, H, KV, hd, at_q=0, at_k=0):
     n = len(q)
     out, pv = (torch.zeros((n, H, hd), dtype=torch.float64, device="cuda") for _ in range(2))
-    size = torch.zeros((n, H), dtype=torch.float64, device="cuda")
+    size, small = torch.zeros((n, H), dtype=torch.float64, device="cuda"), torch.zeros_like(out)
     for a, b in zip(lens_q, lens_k):
         seen = torch.arange(b, device="cuda")[None] <= torch.arange(a, device="cuda")[:, None] + (b - a)
         for h in range(H if a else 0):
@@ -39,9 +39,10 @@ def reference(q, k, v, lens_q, lens_k, H, KV, hd, at_q=0, at_k=0):
             cut = lambda x, lo, m, i: x[lo:lo + m, i * hd:(i + 1) * hd].double()  # noqa: E731
             out[at_q:at_q + a, h], pv[at_q:at_q + a, h], size[at_q:at_q + a, h] = attend(
                 cut(q, at_q, a, h), cut(k, at_k, b, j), cut(v, at_k, b, j), seen)
+            small[at_q:at_q + a, h] = seen.double() @ cut(v, at_k, b, j).abs()
         at_q += a
         at_k += b
-    return out, pv, size
+    return out, (pv, size), small
 
 
 def check(dtype, lens_q, lens_k, H, KV, hd, seed=0, pad=0, scale=1.0, packed=False):
@@ -61,11 +62,11 @@ def check(dtype, lens_q, lens_k, H, KV, hd, seed=0, pad=0, scale=1.0, packed=Fal
     cu_q, cu_k = (i32([0] + np.cumsum(x).tolist()) for x in (lens_q, lens_k))
     err = i32([0])
     call(q, k, v, out[:, :H * hd], cu_q, None if packed else cu_k, len(lens_q), H, KV, hd, err)
-    want, pv, size = reference(q, k, v, lens_q, lens_k, H, KV, hd)
+    want, scores, small = reference(q, k, v, lens_q, lens_k, H, KV, hd)
     n = sum(lens_q)
     assert int(err) == 0
     got = out[:, :H * hd].reshape(-1, H, hd)
-    assert_within(got[:n], want[:n], bound(dtype, want, pv, size, P_ROUND[dtype])[:n], "prompt")
+    assert_within(got[:n], want[:n], bound(dtype, want, *scores, P_ROUND[dtype], small)[:n], "prompt")
     assert bool((out[n:] == 5).all()) and bool((out[:, H * hd:] == 5).all())
     again = torch.full_like(out, 5.0)
     call(q, k, v, again[:, :H * hd], cu_q, None if packed else cu_k, len(lens_q), H, KV, hd, err)
@@ -108,8 +109,8 @@ def test_rising_scores():
     for kk in (k, k.flip(0).contiguous()):
         out = torch.empty_like(q)
         call(q, kk, v, out, i32([0, n]), None, 1, 1, 1, hd)
-        want, pv, size = reference(q, kk, v, [n], [n], 1, 1, hd)
-        assert_within(out.reshape(n, 1, hd), want, bound("bf16", want, pv, size, P_ROUND["bf16"]), "rising")
+        want, scores, _ = reference(q, kk, v, [n], [n], 1, 1, hd)
+        assert_within(out.reshape(n, 1, hd), want, bound("bf16", want, *scores, P_ROUND["bf16"]), "rising")
 
 
 @pytest.mark.parametrize("hd", [64, 128])
