@@ -150,7 +150,11 @@ def test_offsets_past_32_bits():
     x[-3:] = logits(3, V, "bf16", 4)
     _, en, tp, ids = call(x, None, 5)
     _, en3, tp3, ids3 = call(x[-3:].clone(), None, 5)
-    assert torch.equal(en[-3:], en3) and torch.equal(tp[-3:], tp3) and torch.equal(ids[-3:], ids3)
+    # few rows are cut among more CTAs than many, so their sums are taken in another order: each side is
+    # within 2^-18 + 2^-23 |value| (and the entropy's 2^-18 sum p |y|, under 2^-18 * 10 here) of 64 bits
+    assert torch.equal(ids[-3:], ids3)
+    assert bool(((tp[-3:] - tp3).abs() <= 2 * (2.0 ** -18 + 2.0 ** -23 * tp3.abs())).all())
+    assert bool(((en[-3:] - en3).abs() <= 2 * 11 * 2.0 ** -18).all())
 
 
 def test_graph_replay():
