@@ -1,7 +1,7 @@
 // Token log probabilities, entropy and top alternatives (nr_token_logprobs).
 //
 // One read of the logits.  A cluster of 1 to 8 CTAs takes a row, each CTA a run of its
-// 16-byte vectors, each thread every 256th of them: running reference m (moved only when a
+// 32-byte vectors, each thread every 256th of them: running reference m (moved only when a
 // vector's maximum passes it by 8), sum S of e^(x - m) and W of e^(x - m) (x - m), from which
 //
 //   log p(x) = (x - m) - log S,   entropy = log S - W / S.
@@ -21,6 +21,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <cstring>
 
 #include "kv8.h"
 #include "kernels.h"
@@ -36,7 +37,7 @@ constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;       // NR_LOGPROBS_MAX_TOP
 constexpr int kCandidates = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kBatch = 4;         // vectors in flight for each thread
+constexpr int kBatch = 2;         // vectors in flight for each thread
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;
 constexpr float kNothing = -1e4f; // e^-10^4 is 0, and 0 * -10^4 too
@@ -57,50 +58,94 @@ __device__ __forceinline__ float key_value(Key k) {
     return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
-// A row as 16-byte aligned vectors; the first and last may reach over its ends.
+__device__ __forceinline__ __half low_of(__half2 v) { return __low2half(v); }
+__device__ __forceinline__ __half high_of(__half2 v) { return __high2half(v); }
+__device__ __forceinline__ __nv_bfloat16 low_of(__nv_bfloat162 v) { return __low2bfloat16(v); }
+__device__ __forceinline__ __nv_bfloat16 high_of(__nv_bfloat162 v) { return __high2bfloat16(v); }
+
+// A row as 32-byte aligned vectors; the first and last may reach over its ends.
 template <typename T>
 struct RowView {
-    static constexpr int N = 16 / (int)sizeof(T);
+    static constexpr int N = 32 / (int)sizeof(T);
+    struct Vec {
+        uint32_t u[8];
+    };
     const T* p;   // element 0
     int lead;     // elements of vector 0 before it
     int V;
-    __device__ __forceinline__ RowView(const T* row, int v) : p(row), lead((int)((uintptr_t)row % 16 / sizeof(T))), V(v) {}
+    __device__ __forceinline__ RowView(const T* row, int v) : p(row), lead((int)((uintptr_t)row % 32 / sizeof(T))), V(v) {}
     __device__ __forceinline__ int vectors() const { return (int)(((int64_t)V + lead + N - 1) / N); }
     // id of vector i's first element (negative, if it is before the row)
     __device__ __forceinline__ int64_t base(int i) const { return (int64_t)i * N - lead; }
     // elements of vector i, what lies outside the row as -inf
-    __device__ __forceinline__ uint4 load(int i) const {
+    __device__ __forceinline__ Vec load(int i) const {
         const int64_t b = base(i);
+        Vec v;
         if (b >= 0 && b + N <= V) {
-            uint4 u;
-            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p + b));
-            return u;
+            asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(v.u[0]), "=r"(v.u[1]), "=r"(v.u[2]), "=r"(v.u[3]), "=r"(v.u[4]), "=r"(v.u[5]), "=r"(v.u[6]), "=r"(v.u[7])
+                         : "l"(p + b));
+            return v;
         }
-        uint4 u;
-        T* t = reinterpret_cast<T*>(&u);
+        T t[N];
 #pragma unroll
         for (int k = 0; k < N; k++) t[k] = b + k >= 0 && b + k < V ? p[b + k] : from_f32<T>(-INFINITY);
-        return u;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if constexpr (sizeof(T) == 4) {
+                v.u[k] = __float_as_uint(to_f32(t[k]));
+            } else {
+                uint16_t h[2];
+                memcpy(h, &t[2 * k], 4);
+                v.u[k] = h[0] | (uint32_t)h[1] << 16;
+            }
+        }
+        return v;
     }
 };
 
 template <typename T>
-__device__ __forceinline__ void unpack(const uint4& u, float* x) {
-    const T* t = reinterpret_cast<const T*>(&u);
+__device__ __forceinline__ void unpack(const typename RowView<T>::Vec& v, float* x) {
 #pragma unroll
-    for (int k = 0; k < RowView<T>::N; k++) x[k] = to_f32(t[k]);
+    for (int k = 0; k < 8; k++) {
+        if constexpr (std::is_same<T, float>::value) {
+            x[k] = __uint_as_float(v.u[k]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            x[2 * k] = __uint_as_float(v.u[k] << 16);
+            x[2 * k + 1] = __uint_as_float(v.u[k] & 0xffff0000u);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v.u[k]));
+            x[2 * k] = f.x;
+            x[2 * k + 1] = f.y;
+        }
+    }
+}
+
+// The largest element, NaN if there is one.
+template <typename T>
+__device__ __forceinline__ float vec_max(const typename RowView<T>::Vec& v) {
+    if constexpr (std::is_same<T, float>::value) {
+        float t = __uint_as_float(v.u[0]);
+#pragma unroll
+        for (int k = 1; k < 8; k++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(t) : "f"(__uint_as_float(v.u[k])));
+        return t;
+    } else {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        T2 t[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) t[k] = *reinterpret_cast<const T2*>(&v.u[k]);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+            for (int k = 0; k < o; k++) t[k] = __hmax2_nan(t[k], t[k + o]);
+        return to_f32(__hmax_nan(low_of(t[0]), high_of(t[0])));
+    }
 }
 
 struct Stats {
@@ -121,31 +166,47 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
     return {m, a.s + b.s, a.w + b.w};
 }
 
-// One vector of N values into a thread's running sums.
-template <int N>
-__device__ __forceinline__ void take(const float* x, float top, Stats& a) {
-    if (top > a.m + kLazy) a = moved(a, top);
-    const float m = a.m == -INFINITY ? 0.0f : a.m;
+// Sums of one vector's N values.  e^-inf * -inf is NaN: with CLAMP such values count as
+// nothing, without it the weighted sum tells that there is one.
+template <int N, bool CLAMP>
+__device__ __forceinline__ void sums_of(const float* x, float m, float& s, float& w) {
     const unsigned long long m2 = pack2(__float_as_uint(m), __float_as_uint(m));
-    const unsigned long long log2e = pack2(__float_as_uint(kLog2e), __float_as_uint(kLog2e));
-    unsigned long long s = 0, w = 0;
+    const unsigned long long l2 = pack2(__float_as_uint(kLog2e), __float_as_uint(kLog2e));
+    unsigned long long ss = 0, ww = 0;
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
-        uint32_t d0, d1, y0, y1;
-        unpack2(sub2(pack2(__float_as_uint(x[k]), __float_as_uint(x[k + 1])), m2), d0, d1);
-        const unsigned long long d = pack2(__float_as_uint(fmaxf(__uint_as_float(d0), kNothing)),
-                                           __float_as_uint(fmaxf(__uint_as_float(d1), kNothing)));
-        unpack2(mul2(d, log2e), y0, y1);
-        const unsigned long long e = pack2(__float_as_uint(exp2_fast(__uint_as_float(y0))),
-                                           __float_as_uint(exp2_fast(__uint_as_float(y1))));
-        s = k ? add2(s, e) : e;
-        w = fma2(e, d, w);
+        unsigned long long d = sub2(pack2(__float_as_uint(x[k]), __float_as_uint(x[k + 1])), m2);
+        uint32_t a, b;
+        if (CLAMP) {
+            unpack2(d, a, b);
+            d = pack2(__float_as_uint(fmaxf(__uint_as_float(a), kNothing)), __float_as_uint(fmaxf(__uint_as_float(b), kNothing)));
+        }
+        unpack2(mul2(d, l2), a, b);
+        const unsigned long long e = pack2(__float_as_uint(exp2_fast(__uint_as_float(a))),
+                                           __float_as_uint(exp2_fast(__uint_as_float(b))));
+        ss = k ? add2(ss, e) : e;
+        ww = k ? fma2(e, d, ww) : mul2(e, d);
     }
-    uint32_t s0, s1, w0, w1;
-    unpack2(s, s0, s1);
-    unpack2(w, w0, w1);
-    a.s += __uint_as_float(s0) + __uint_as_float(s1);
-    a.w += __uint_as_float(w0) + __uint_as_float(w1);
+    uint32_t a, b;
+    unpack2(ss, a, b);
+    s = __uint_as_float(a) + __uint_as_float(b);
+    unpack2(ww, a, b);
+    w = __uint_as_float(a) + __uint_as_float(b);
+}
+
+// One vector into a thread's running sums; `masked`: whether it has met a -inf.
+template <int N>
+__device__ __forceinline__ void take(const float* x, float top, Stats& a, bool& masked) {
+    if (top > a.m + kLazy) a = moved(a, top);
+    const float m = a.m == -INFINITY ? 0.0f : a.m;
+    float s, w = NAN;
+    if (!masked) sums_of<N, false>(x, m, s, w);
+    if (w != w) {
+        masked = true;
+        sums_of<N, true>(x, m, s, w);
+    }
+    a.s += s;
+    a.w += w;
 }
 
 struct Shared {
@@ -223,28 +284,27 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
     Stats st{-INFINITY, 0.0f, 0.0f};
     float best = -INFINITY;
     int best_v = v0 + t;
-    bool nan = false;
-    auto fetch = [&](uint4* u, int v) {
+    bool nan = false, masked = false;
+    using Vec = typename RowView<T>::Vec;
+    auto fetch = [&](Vec* u, int v) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++)
             if (v + i * kThreads < v1) u[i] = row.load(v + i * kThreads);
     };
-    auto use = [&](const uint4* u, int v) {
+    auto use = [&](const Vec* u, int v) {
 #pragma unroll
         for (int i = 0; i < kBatch; i++) {
             if (v + i * kThreads >= v1) break;
+            const float top = vec_max<T>(u[i]);
             float x[N];
             unpack<T>(u[i], x);
-            float top = x[0];
-#pragma unroll
-            for (int k = 1; k < N; k++) top = max_nan(top, x[k]);
             nan |= top != top;
             if (top > best) best = top, best_v = v + i * kThreads;
-            take<N>(x, top, st);
+            take<N>(x, top, st, masked);
         }
     };
     {
-        uint4 u[2][kBatch];
+        Vec u[2][kBatch];
         const int step = kBatch * kThreads;
         fetch(u[0], v0 + t);
         for (int v = v0 + t; v < v1; v += 2 * step) {
@@ -345,18 +405,19 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
         all = sh.all;
     }
     __syncthreads();
-    const float ls = all.s > 0.0f || all.s != all.s ? logf(all.s) : NAN;
+    const float ls = all.s > 0.0f ? logf(all.s) : NAN;
+    auto logprob = [&](float x) { return (x - all.m) - ls; };
     if (t == 0) {
         if (a.targets) {
             const int id = a.targets[m_row];
-            a.target_logprob[m_row] = id < 0 || id >= a.V ? NAN : (to_f32(row.p[id]) - all.m) - ls;
+            a.target_logprob[m_row] = id < 0 || id >= a.V ? NAN : logprob(to_f32(row.p[id]));
         }
         if (a.entropy) a.entropy[m_row] = ls - all.w / all.s;
     }
     if (t < k) {
         const Key key = list[t];
         a.top_ids[m_row * k + t] = key_number(key);
-        a.top_logprob[m_row * k + t] = (key_value(key) - all.m) - ls;
+        a.top_logprob[m_row * k + t] = logprob(key_value(key));
     }
 }
 
