@@ -9,14 +9,15 @@
 // x - m is taken before the factor log2 e, so that large logits keep their differences.
 //
 // Top k without a second pass: every thread also keeps its largest vector maximum.  With the
-// keys (value, vector number) ordered by larger value, then smaller number, let K be the k-th
-// largest thread key.  k elements are as large as K or larger, so every element of the top k
-// is, and such elements are found in those k threads' vectors alone: only these (1/8 of the
-// row at k = 32) are looked at again, while they are in L2.  The few candidates are ranked by
-// counting the larger ones (ids make all keys distinct, so equal logits fall in order of their
-// ids), the lists of a cluster's CTAs are joined the same way through distributed shared
-// memory.  Rows that hold a NaN or +inf and more candidates than the buffer holds take k
-// passes instead.
+// keys (value, vector number) ordered by larger value, then smaller number, let K be the
+// smallest, over the CTA's w full warps, of a warp's ceil(k/w)-th largest thread key.  Then k
+// elements at least are as large as K or larger, so every element of the top k is, and such
+// elements are found only in vectors of the few threads whose key is: the thread's best one,
+// and all of them if its second largest maximum is as large as K, are looked at again while
+// they are in L2.  The candidates are ranked by counting the larger ones (ids
+// make all keys distinct, so equal logits fall in order of their ids), the lists of a
+// cluster's CTAs are joined the same way through distributed shared memory.  Rows that hold a
+// NaN and more candidates than the buffer holds take k passes instead.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -37,7 +38,6 @@ constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;       // NR_LOGPROBS_MAX_TOP
 constexpr int kCandidates = 1024;
 constexpr int kMaxCluster = 8;
-constexpr int kBatch = 2;         // vectors in flight for each thread
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.0f;
 constexpr float kNothing = -1e4f; // e^-10^4 is 0, and 0 * -10^4 too
@@ -83,16 +83,21 @@ struct RowView {
     __device__ __forceinline__ int vectors() const { return (int)(((int64_t)V + lead + N - 1) / N); }
     // id of vector i's first element (negative, if it is before the row)
     __device__ __forceinline__ int64_t base(int i) const { return (int64_t)i * N - lead; }
-    // elements of vector i, what lies outside the row as -inf
-    __device__ __forceinline__ Vec load(int i) const {
+    // vectors that lie inside the row
+    __device__ __forceinline__ int first_whole() const { return lead ? 1 : 0; }
+    __device__ __forceinline__ int end_whole() const { return (int)(((int64_t)V + lead) / N); }
+    __device__ __forceinline__ Vec load_whole(int i) const { return load_whole_at(p + base(i)); }
+    static __device__ __forceinline__ Vec load_whole_at(const T* at) {
+        Vec v;
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(v.u[0]), "=r"(v.u[1]), "=r"(v.u[2]), "=r"(v.u[3]), "=r"(v.u[4]), "=r"(v.u[5]), "=r"(v.u[6]), "=r"(v.u[7])
+                     : "l"(at));
+        return v;
+    }
+    // elements of any vector i, what lies outside the row as -inf
+    __device__ __noinline__ Vec load(int i) const {
         const int64_t b = base(i);
         Vec v;
-        if (b >= 0 && b + N <= V) {
-            asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                         : "=r"(v.u[0]), "=r"(v.u[1]), "=r"(v.u[2]), "=r"(v.u[3]), "=r"(v.u[4]), "=r"(v.u[5]), "=r"(v.u[6]), "=r"(v.u[7])
-                         : "l"(p + b));
-            return v;
-        }
         T t[N];
 #pragma unroll
         for (int k = 0; k < N; k++) t[k] = b + k >= 0 && b + k < V ? p[b + k] : from_f32<T>(-INFINITY);
@@ -170,39 +175,31 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
 // nothing, without it the weighted sum tells that there is one.
 template <int N, bool CLAMP>
 __device__ __forceinline__ void sums_of(const float* x, float m, float& s, float& w) {
-    const unsigned long long m2 = pack2(__float_as_uint(m), __float_as_uint(m));
-    const unsigned long long l2 = pack2(__float_as_uint(kLog2e), __float_as_uint(kLog2e));
-    unsigned long long ss = 0, ww = 0;
+    float ss[2] = {0.0f, 0.0f}, ww[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < N; k += 2) {
-        unsigned long long d = sub2(pack2(__float_as_uint(x[k]), __float_as_uint(x[k + 1])), m2);
-        uint32_t a, b;
-        if (CLAMP) {
-            unpack2(d, a, b);
-            d = pack2(__float_as_uint(fmaxf(__uint_as_float(a), kNothing)), __float_as_uint(fmaxf(__uint_as_float(b), kNothing)));
-        }
-        unpack2(mul2(d, l2), a, b);
-        const unsigned long long e = pack2(__float_as_uint(exp2_fast(__uint_as_float(a))),
-                                           __float_as_uint(exp2_fast(__uint_as_float(b))));
-        ss = k ? add2(ss, e) : e;
-        ww = k ? fma2(e, d, ww) : mul2(e, d);
+    for (int k = 0; k < N; k++) {
+        float d = x[k] - m;
+        if (CLAMP) d = fmaxf(d, kNothing);
+        const float e = exp2_fast(d * kLog2e);
+        ss[k & 1] += e;
+        ww[k & 1] = fmaf(e, d, ww[k & 1]);
     }
-    uint32_t a, b;
-    unpack2(ss, a, b);
-    s = __uint_as_float(a) + __uint_as_float(b);
-    unpack2(ww, a, b);
-    w = __uint_as_float(a) + __uint_as_float(b);
+    s = ss[0] + ss[1];
+    w = ww[0] + ww[1];
 }
 
-// One vector into a thread's running sums; `masked`: whether it has met a -inf.
+// One vector into a thread's running sums; `masked`: whether it has met a -inf, `nan` a NaN.
 template <int N>
-__device__ __forceinline__ void take(const float* x, float top, Stats& a, bool& masked) {
+__device__ __forceinline__ void take(const float* x, float top, Stats& a, bool& masked, bool& nan) {
     if (top > a.m + kLazy) a = moved(a, top);
     const float m = a.m == -INFINITY ? 0.0f : a.m;
-    float s, w = NAN;
-    if (!masked) sums_of<N, false>(x, m, s, w);
-    if (w != w) {
-        masked = true;
+    float s, w;
+    if (!masked) {
+        sums_of<N, false>(x, m, s, w);
+        masked = w != w;
+    }
+    if (masked) {
+        nan |= top != top;
         sums_of<N, true>(x, m, s, w);
     }
     a.s += s;
@@ -214,13 +211,11 @@ struct Shared {
     Stats all;             // of the CTA
     int bad;               // a NaN in the CTA's part
     int count;             // candidates
-    int chosen[kMaxTop];   // threads whose vectors are looked at again
-    Key bound;
+    int n_chosen;
+    int chosen[kThreads];  // threads whose vectors are looked at again
+    Key warp_key[kThreads / 32];
     Key top[kMaxTop];      // the CTA's list
-    union {
-        Key keys[kCandidates];
-        Key thread_key[kThreads];
-    };
+    Key keys[kCandidates];
 };
 
 // Ranks the n distinct keys and writes the first k of them in order.
@@ -282,37 +277,42 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
 
     // the pass over this CTA's vectors
     Stats st{-INFINITY, 0.0f, 0.0f};
-    float best = -INFINITY;
+    float best = -INFINITY, second = -INFINITY;
     int best_v = v0 + t;
     bool nan = false, masked = false;
     using Vec = typename RowView<T>::Vec;
-    auto fetch = [&](Vec* u, int v) {
-#pragma unroll
-        for (int i = 0; i < kBatch; i++)
-            if (v + i * kThreads < v1) u[i] = row.load(v + i * kThreads);
-    };
-    auto use = [&](const Vec* u, int v) {
-#pragma unroll
-        for (int i = 0; i < kBatch; i++) {
-            if (v + i * kThreads >= v1) break;
-            const float top = vec_max<T>(u[i]);
-            float x[N];
-            unpack<T>(u[i], x);
-            nan |= top != top;
-            if (top > best) best = top, best_v = v + i * kThreads;
-            take<N>(x, top, st, masked);
-        }
+    const int w0 = row.first_whole(), w1 = min(v1, row.end_whole());
+    auto use = [&](const Vec& u, int v) {
+        const float top = vec_max<T>(u);
+        float x[N];
+        unpack<T>(u, x);
+        second = fmaxf(second, fminf(top, best));
+        if (top > best) best = top, best_v = v;
+        take<N>(x, top, st, masked, nan);
     };
     {
-        Vec u[2][kBatch];
-        const int step = kBatch * kThreads;
-        fetch(u[0], v0 + t);
-        for (int v = v0 + t; v < v1; v += 2 * step) {
-            fetch(u[1], v + step);
-            use(u[0], v);
-            fetch(u[0], v + 2 * step);
-            use(u[1], v + step);
+        // a thread's first and last vector may reach over the row's ends, the others are whole
+        int v = v0 + t;
+        if (v < v1 && v < w0) use(row.load(v), v), v += kThreads;
+        const int n = w1 > v ? (w1 - v + kThreads - 1) / kThreads : 0;
+        const T* p = row.p + row.base(v);
+        auto whole = [&](int i) { return row.load_whole_at(p + (int64_t)i * (kThreads * N)); };
+        Vec a, b;
+        if (n > 0) a = whole(0);
+        if (n > 1) b = whole(1);
+        int i = 0;
+        for (; i + 3 < n; i += 2) {
+            use(a, v + i * kThreads);
+            a = whole(i + 2);
+            use(b, v + (i + 1) * kThreads);
+            b = whole(i + 3);
         }
+        if (i < n) use(a, v + i * kThreads);
+        if (i + 2 < n) a = whole(i + 2);
+        if (i + 1 < n) use(b, v + (i + 1) * kThreads);
+        if (i + 2 < n) use(a, v + (i + 2) * kThreads);
+        const int edge = nv - 1;
+        if (edge >= w1 && edge >= max(v0, w0) && edge < v1 && (edge - v0) % kThreads == t) use(row.load(edge), edge);
     }
 
     // the CTA's sums
@@ -325,8 +325,22 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
     }
     const int k = a.top_k;
     if (lane == 0) sh.stats[t >> 5] = sum;
-    if (t == 0) sh.count = 0, sh.bound = 0;
-    if (k) sh.thread_key[t] = v0 + t < v1 ? rank_key(best, best_v) : 0;
+    if (t == 0) sh.count = sh.n_chosen = 0;
+    const Key mine = k && v0 + t < v1 ? rank_key(best, best_v) : 0;
+    const int full = min(kThreads, v1 - v0) / 32;  // warps whose every thread has vectors
+    if (k && (t >> 5) < full) {
+        Key left = mine, top = 0;
+        for (int r = 0; r < (k + full - 1) / full; r++) {
+            top = left;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const Key q = __shfl_xor_sync(0xffffffffu, top, o);
+                top = q > top ? q : top;
+            }
+            if (left == top) left = 0;
+        }
+        if (lane == 0) sh.warp_key[t >> 5] = top;
+    }
     const bool bad = __syncthreads_or(nan);
     if (t < 32) {
         sum = lane < kThreads / 32 ? sh.stats[lane] : Stats{-INFINITY, 0.0f, 0.0f};
@@ -345,31 +359,36 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
 
     // the CTA's top k
     if (k) {
-        const Key mine = sh.thread_key[t];
-        int larger = 0;
-#pragma unroll 8
-        for (int j = 0; j < kThreads; j += 2) {
-            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(&sh.thread_key[j]);
-            larger += (q.x > mine) + (q.y > mine);
+        Key bound = full ? ~0ull : 0;  // fewer than 32 vectors: all their elements
+        for (int w = 0; w < full; w++) bound = sh.warp_key[w] < bound ? sh.warp_key[w] : bound;
+        const float least = bound ? key_value(bound) : -INFINITY;
+        auto look = [&](int v) {
+            const Vec u = v >= w0 && v < w1 ? row.load_whole(v) : row.load(v);
+            if (vec_max<T>(u) < least) return;
+            float x[N];
+            unpack<T>(u, x);
+            uint32_t hits = 0;
+#pragma unroll
+            for (int e = 0; e < N; e++) hits |= (x[e] >= least ? 1u : 0u) << e;
+            for (; hits; hits &= hits - 1) {
+                const int e = __ffs(hits) - 1;
+                const int64_t id = row.base(v) + e;
+                if (id < 0 || id >= a.V) continue;
+                const float value = to_f32(row.p[id]);
+                if (rank_key(value, v) < bound) continue;
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < kCandidates) sh.keys[at] = rank_key(value, (int)id);
+            }
+        };
+        if (!bad && mine && mine >= bound) {
+            if (second >= least) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = t;
+            else look(best_v);
         }
-        if (mine && larger < k) sh.chosen[larger] = t;
-        if (larger == k - 1 && mine) sh.bound = mine;  // stays 0 where fewer than k threads have vectors
-        const int chosen = min(k, min(kThreads, v1 - v0));
         __syncthreads();
         if (!bad) {
-            const Key bound = sh.bound;
+            const int chosen = sh.n_chosen;
             for (int c = t >> 5; c < chosen; c += kThreads / 32)
-                for (int v = v0 + sh.chosen[c] + lane * kThreads; v < v1; v += 32 * kThreads) {
-                    float x[N];
-                    unpack<T>(row.load(v), x);
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const int64_t id = row.base(v) + e;
-                        if (id < 0 || id >= a.V || rank_key(x[e], v) < bound) continue;
-                        const int at = atomicAdd(&sh.count, 1);
-                        if (at < kCandidates) sh.keys[at] = rank_key(x[e], (int)id);
-                    }
-                }
+                for (int v = v0 + sh.chosen[c] + lane * kThreads; v < v1; v += 32 * kThreads) look(v);
         }
         __syncthreads();
         if (t < k) sh.top[t] = 0;
