@@ -12,12 +12,19 @@
 // keys (value, vector number) ordered by larger value, then smaller number, let K be the
 // smallest, over the CTA's w full warps, of a warp's ceil(k/w)-th largest thread key.  Then k
 // elements at least are as large as K or larger, so every element of the top k is, and such
-// elements are found only in vectors of the few threads whose key is: the thread's best one,
-// and all of them if its second largest maximum is as large as K, are looked at again while
-// they are in L2.  The candidates are ranked by counting the larger ones (ids
+// elements are found only in vectors of the few threads whose key is: the thread's two best
+// ones, and all of them if its third largest maximum is as large as K, are looked at again
+// while they are in L2.  The candidates are ranked by counting the larger ones (ids
 // make all keys distinct, so equal logits fall in order of their ids), the lists of a
 // cluster's CTAs are joined the same way through distributed shared memory.  Rows that hold a
 // NaN and more candidates than the buffer holds take k passes instead.
+//
+// Measured: 2048 rows of 128256 bf16 logits, top 20: 114 us, 4.63 TB/s, 0.71 of the measured copy
+// bandwidth (100 us without a top list; fp32 logits 6.0 TB/s, 0.92): two elements of 16 bits
+// for each of 32 need twice the exponentials (8 cycles a warp) and sums for the same bytes,
+// and the candidates' latency is hidden only by the SM's other rows.  64 rows of 32000 fp32:
+// 9.2 us, a chain of latencies.  A ninth warp that finishes a row while the others stream
+// the next one was slower (140 us: fewer registers and a longer chain on one warp).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -171,14 +178,29 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
     return {m, a.s + b.s, a.w + b.w};
 }
 
-// Sums of one vector's N values.  e^-inf * -inf is NaN: with CLAMP such values count as
-// nothing, without it the weighted sum tells that there is one.
-template <int N, bool CLAMP>
-__device__ __forceinline__ void sums_of(const float* x, float m, float& s, float& w) {
+// x - m of one element; the 16-bit types' subtraction widens its operand itself.
+__device__ __forceinline__ float less(uint32_t x, float m, float) { return __uint_as_float(x) - m; }
+__device__ __forceinline__ float less(uint16_t x, float m, __nv_bfloat16) {
+    float d;
+    asm("sub.rn.f32.bf16 %0, %1, %2;" : "=f"(d) : "h"(x), "f"(m));
+    return d;
+}
+__device__ __forceinline__ float less(uint16_t x, float m, __half) {
+    float d;
+    asm("sub.rn.f32.f16 %0, %1, %2;" : "=f"(d) : "h"(x), "f"(m));
+    return d;
+}
+
+// Sums of one vector.  e^-inf * -inf is NaN: with CLAMP such values count as nothing, without
+// it the weighted sum tells that there is one.
+template <typename T, bool CLAMP>
+__device__ __forceinline__ void sums_of(const typename RowView<T>::Vec& v, float m, float& s, float& w) {
     float ss[2] = {0.0f, 0.0f}, ww[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-        float d = x[k] - m;
+    for (int k = 0; k < RowView<T>::N; k++) {
+        float d;
+        if constexpr (sizeof(T) == 4) d = less(v.u[k], m, T());
+        else d = less((uint16_t)(v.u[k / 2] >> (16 * (k & 1))), m, T());
         if (CLAMP) d = fmaxf(d, kNothing);
         const float e = exp2_fast(d * kLog2e);
         ss[k & 1] += e;
@@ -189,18 +211,18 @@ __device__ __forceinline__ void sums_of(const float* x, float m, float& s, float
 }
 
 // One vector into a thread's running sums; `masked`: whether it has met a -inf, `nan` a NaN.
-template <int N>
-__device__ __forceinline__ void take(const float* x, float top, Stats& a, bool& masked, bool& nan) {
+template <typename T>
+__device__ __forceinline__ void take(const typename RowView<T>::Vec& v, float top, Stats& a, bool& masked, bool& nan) {
     if (top > a.m + kLazy) a = moved(a, top);
     const float m = a.m == -INFINITY ? 0.0f : a.m;
     float s, w;
     if (!masked) {
-        sums_of<N, false>(x, m, s, w);
+        sums_of<T, false>(v, m, s, w);
         masked = w != w;
     }
     if (masked) {
         nan |= top != top;
-        sums_of<N, true>(x, m, s, w);
+        sums_of<T, true>(v, m, s, w);
     }
     a.s += s;
     a.w += w;
@@ -218,14 +240,11 @@ struct Shared {
     Key keys[kCandidates];
 };
 
-// Ranks the n distinct keys and writes the first k of them in order.
-__device__ __forceinline__ void rank_keys(const Key* keys, int n, int k, Key* out) {
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const Key mine = keys[i];
-        int larger = 0;
-        for (int j = 0; j < n; j++) larger += keys[j] > mine;
-        if (larger < k) out[larger] = mine;
-    }
+// Largest key of the warp.
+__device__ __forceinline__ Key warp_max_key(Key k) {
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+    return ((Key)hi << 32) | lo;
 }
 
 // The k largest keys of vectors v0 .. v1 - 1, one pass for each.
@@ -263,10 +282,9 @@ __device__ void top_by_passes(const RowView<T>& row, int v0, int v1, int k, Shar
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cluster) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 5) logprob_kernel(LogprobArgs a, int cluster) {
     constexpr int N = RowView<T>::N;
     __shared__ Shared sh;
-    __shared__ Key lists[kMaxCluster * kMaxTop];
     const int t = threadIdx.x, lane = t & 31, rank = blockIdx.x % cluster;
     const int64_t m_row = blockIdx.x / cluster;
     grid_dependency_wait();
@@ -275,20 +293,22 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
     const int nv = row.vectors(), per = (nv + cluster - 1) / cluster;
     const int v0 = min(rank * per, nv), v1 = min(nv, v0 + per);
 
+    if (t < kMaxTop) sh.top[t] = 0;
+    if (t == 0) sh.count = sh.n_chosen = 0;
+
     // the pass over this CTA's vectors
     Stats st{-INFINITY, 0.0f, 0.0f};
-    float best = -INFINITY, second = -INFINITY;
-    int best_v = v0 + t;
+    float best = -INFINITY, second = -INFINITY, third = -INFINITY;
+    int best_v = v0 + t, second_v = -1;
     bool nan = false, masked = false;
     using Vec = typename RowView<T>::Vec;
     const int w0 = row.first_whole(), w1 = min(v1, row.end_whole());
     auto use = [&](const Vec& u, int v) {
         const float top = vec_max<T>(u);
-        float x[N];
-        unpack<T>(u, x);
-        second = fmaxf(second, fminf(top, best));
-        if (top > best) best = top, best_v = v;
-        take<N>(x, top, st, masked, nan);
+        third = fmaxf(third, fminf(top, second));
+        if (top > best) second = best, second_v = best_v, best = top, best_v = v;
+        else if (top > second) second = top, second_v = v;
+        take<T>(u, top, st, masked, nan);
     };
     {
         // a thread's first and last vector may reach over the row's ends, the others are whole
@@ -325,18 +345,12 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
     }
     const int k = a.top_k;
     if (lane == 0) sh.stats[t >> 5] = sum;
-    if (t == 0) sh.count = sh.n_chosen = 0;
     const Key mine = k && v0 + t < v1 ? rank_key(best, best_v) : 0;
     const int full = min(kThreads, v1 - v0) / 32;  // warps whose every thread has vectors
     if (k && (t >> 5) < full) {
         Key left = mine, top = 0;
         for (int r = 0; r < (k + full - 1) / full; r++) {
-            top = left;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const Key q = __shfl_xor_sync(0xffffffffu, top, o);
-                top = q > top ? q : top;
-            }
+            top = warp_max_key(left);
             if (left == top) left = 0;
         }
         if (lane == 0) sh.warp_key[t >> 5] = top;
@@ -362,68 +376,79 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
         Key bound = full ? ~0ull : 0;  // fewer than 32 vectors: all their elements
         for (int w = 0; w < full; w++) bound = sh.warp_key[w] < bound ? sh.warp_key[w] : bound;
         const float least = bound ? key_value(bound) : -INFINITY;
-        auto look = [&](int v) {
-            const Vec u = v >= w0 && v < w1 ? row.load_whole(v) : row.load(v);
-            if (vec_max<T>(u) < least) return;
+        auto look = [&](const Vec& u, int v) {
+            uint32_t hits = 0;
             float x[N];
             unpack<T>(u, x);
-            uint32_t hits = 0;
 #pragma unroll
             for (int e = 0; e < N; e++) hits |= (x[e] >= least ? 1u : 0u) << e;
             for (; hits; hits &= hits - 1) {
                 const int e = __ffs(hits) - 1;
                 const int64_t id = row.base(v) + e;
-                if (id < 0 || id >= a.V) continue;
-                const float value = to_f32(row.p[id]);
-                if (rank_key(value, v) < bound) continue;
+                float value = x[0];
+#pragma unroll
+                for (int j = 1; j < N; j++) value = e == j ? x[j] : value;
+                if (id < 0 || id >= a.V || rank_key(value, v) < bound) continue;
                 const int at = atomicAdd(&sh.count, 1);
                 if (at < kCandidates) sh.keys[at] = rank_key(value, (int)id);
             }
         };
+        auto any = [&](int v) { return v >= w0 && v < w1 ? row.load_whole(v) : row.load(v); };
         if (!bad && mine && mine >= bound) {
-            if (second >= least) sh.chosen[atomicAdd(&sh.n_chosen, 1)] = t;
-            else look(best_v);
+            if (third >= least) {
+                sh.chosen[atomicAdd(&sh.n_chosen, 1)] = t;
+            } else {
+                const bool two = second_v >= 0 && second >= least;
+                const Vec x = any(best_v), y = any(two ? second_v : best_v);
+                look(x, best_v);
+                if (two) look(y, second_v);
+            }
         }
         __syncthreads();
-        if (!bad) {
-            const int chosen = sh.n_chosen;
+        const int chosen = sh.n_chosen;
+        if (chosen) {
             for (int c = t >> 5; c < chosen; c += kThreads / 32)
-                for (int v = v0 + sh.chosen[c] + lane * kThreads; v < v1; v += 32 * kThreads) look(v);
+                for (int v = v0 + sh.chosen[c] + lane * kThreads; v < v1; v += 32 * kThreads) look(any(v), v);
+            __syncthreads();
         }
-        __syncthreads();
-        if (t < k) sh.top[t] = 0;
-        __syncthreads();
-        if (bad || sh.count > kCandidates) top_by_passes(row, v0, v1, k, sh);
-        else rank_keys(sh.keys, sh.count, k, sh.top);
+        if (bad || sh.count > kCandidates) {
+            top_by_passes(row, v0, v1, k, sh);
+        } else {
+            // four threads to a candidate
+            const int n = sh.count;
+            for (int i = t / 4; i < (n + 7) / 8 * 8; i += kThreads / 4) {
+                const Key key = i < n ? sh.keys[i] : 0;
+                int larger = 0;
+                for (int j = t % 4; j < n; j += 4) larger += sh.keys[j] > key;
+                larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+                larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+                if (i < n && larger < k && t % 4 == 0) sh.top[larger] = key;
+            }
+        }
     }
 
-    // the cluster's
-    Stats all;
-    const Key* list = sh.top;
+    __syncthreads();
+    Stats all = sh.all;
+    Key key = t < k ? sh.top[t] : 0;
     if (cluster > 1) {
+        // the first CTA's first warp joins the parts: lane c has list c, which is in order, and
+        // the largest head is taken k times
         cg::cluster_group cl = cg::this_cluster();
         cl.sync();
-        if (rank == 0) {
-            all = sh.all;
+        if (rank == 0 && t < 32) {
             for (int r = 1; r < cluster; r++) all = join(all, cl.map_shared_rank(&sh, r)->all);
-            for (int i = t; i < cluster * k; i += kThreads) lists[i] = cl.map_shared_rank(&sh, i / k)->top[i % k];
+            const Shared* theirs = cl.map_shared_rank(&sh, min(lane, cluster - 1));
+            Key head = lane < cluster && k ? theirs->top[0] : 0;
+            int at = 0;
+            for (int i = 0; i < k; i++) {
+                const Key top = warp_max_key(head);
+                if (lane == i) key = top;
+                if (head == top && head) head = ++at < k ? theirs->top[at] : 0;
+            }
         }
         cl.sync();  // no CTA leaves while its list is read
         if (rank) return;
-        if (k) {
-            // absent entries are 0: they rank behind every key, in any order
-            for (int i = t; i < cluster * k; i += kThreads) {
-                const Key mine = lists[i];
-                int larger = 0;
-                for (int j = 0; j < cluster * k; j++) larger += lists[j] > mine;
-                if (mine && larger < k) sh.top[larger] = mine;
-            }
-        }
-    } else {
-        __syncthreads();
-        all = sh.all;
     }
-    __syncthreads();
     const float ls = all.s > 0.0f ? logf(all.s) : NAN;
     auto logprob = [&](float x) { return (x - all.m) - ls; };
     if (t == 0) {
@@ -434,7 +459,6 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
         if (a.entropy) a.entropy[m_row] = ls - all.w / all.s;
     }
     if (t < k) {
-        const Key key = list[t];
         a.top_ids[m_row * k + t] = key_number(key);
         a.top_logprob[m_row * k + t] = logprob(key_value(key));
     }
@@ -442,11 +466,13 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int cl
 
 template <typename T>
 cudaError_t launch_t(const LogprobArgs& a, cudaStream_t s) {
-    // More CTAs to a row while it has over 4096 elements for each and they all fit the device at
-    // once: few rows are bound by latency, many by memory, where a CTA for each row has the
-    // least to join.
+    // More CTAs to a row while it has over 4096 elements for each and the grid stays within two
+    // CTAs to an SM: few rows are bound by latency (1 x 32000: 8.4 us with one CTA, 6.8 with 8;
+    // 16 x 128256: 15.8, 9.7), more of them by what each CTA has to join (64 x 32000: 9.1 us
+    // with 4, 10.4 with 8; 128 x 128256: 21.6, 17.8, 19.5 with 1, 2, 4), many by memory (2048 x
+    // 128256: 114 us with 1, 150 with 2).
     int cluster = 1;
-    while (cluster < kMaxCluster && a.V / cluster > 4096 && (int64_t)a.M * cluster * 2 <= 148 * 4) cluster *= 2;
+    while (cluster < kMaxCluster && a.V / cluster > 4096 && (int64_t)a.M * cluster <= 148) cluster *= 2;
     count_launch();
     return launch_ex(logprob_kernel<T>, dim3((unsigned)((int64_t)a.M * cluster)), dim3(kThreads), 0, s, (unsigned)cluster, a, cluster);
 }
