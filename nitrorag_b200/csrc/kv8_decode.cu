@@ -41,8 +41,14 @@ namespace nitro {
 namespace {
 
 constexpr int kWarps = 4;
-// Units to cut a batch into: three CTAs are resident on each of 148 SMs.
-constexpr int kUnits = 3 * 148;
+constexpr int kWaves = 4;
+constexpr int kSms = 148, kMostCtas = 4;
+// Pages are cut into so many units, `slots` of which run at once.  With few items the last
+// units should not start a second wave (each item can add one unit to the even cut); many
+// items run in several waves anyway, which smaller units even out.
+__host__ __device__ __forceinline__ int units_wanted(int64_t items, int slots) {
+    return items <= slots / 2 ? slots - (int)items : kWaves * slots;
+}
 constexpr int kMinPages = 8;            // of a unit: two for each warp
 // Items whose partial results can be counted; more items than that fill the device uncut.
 constexpr int kCounters = 16384;
@@ -108,29 +114,34 @@ __device__ __forceinline__ float gain_of(float x) {
     return __uint_as_float((uint32_t)min(max(261 - e, 2), 252) << 23);
 }
 
-// A lane's part of one page: with g = lane / 4, c = lane % 4, bytes 16c.. of each 64 of K's
-// rows g and g + 8, and bytes g*HD/8.. of V's rows 2c, 2c+1, 2c+8, 2c+9.
+// A lane's part of a page of K and of V: with g = lane / 4, c = lane % 4, bytes 16c.. of each
+// 64 of K's rows g and g + 8, and bytes g*HD/8.. of V's rows 2c, 2c+1, 2c+8, 2c+9.
 template <int HD>
-struct PageRegs {
-    uint32_t k[2][HD / 64][4];
-    uint32_t v[4][HD / 32];
-    __device__ __forceinline__ void load(const uint8_t* kt, const uint8_t* vt, int g, int c) {
+struct KeyRegs {
+    uint32_t w[2][HD / 64][4];
+    __device__ __forceinline__ void load(const uint8_t* tile, int g, int c) {
 #pragma unroll
         for (int r = 0; r < 2; r++)
 #pragma unroll
             for (int j = 0; j < HD / 64; j++) {
-                const uint4 u = load16(kt + (g + 8 * r) * HD + 64 * j + 16 * c);
-                k[r][j][0] = u.x; k[r][j][1] = u.y; k[r][j][2] = u.z; k[r][j][3] = u.w;
+                const uint4 u = load16(tile + (g + 8 * r) * HD + 64 * j + 16 * c);
+                w[r][j][0] = u.x; w[r][j][1] = u.y; w[r][j][2] = u.z; w[r][j][3] = u.w;
             }
+    }
+};
+template <int HD>
+struct ValueRegs {
+    uint32_t w[4][HD / 32];
+    __device__ __forceinline__ void load(const uint8_t* tile, int g, int c) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            const uint8_t* p = vt + (2 * c + (t & 1) + 8 * (t >> 1)) * HD + g * (HD / 8);
+            const uint8_t* p = tile + (2 * c + (t & 1) + 8 * (t >> 1)) * HD + g * (HD / 8);
             if constexpr (HD == 128) {
                 const uint4 u = load16(p);
-                v[t][0] = u.x; v[t][1] = u.y; v[t][2] = u.z; v[t][3] = u.w;
+                w[t][0] = u.x; w[t][1] = u.y; w[t][2] = u.z; w[t][3] = u.w;
             } else {
                 const uint2 u = load8(p);
-                v[t][0] = u.x; v[t][1] = u.y;
+                w[t][0] = u.x; w[t][1] = u.y;
             }
         }
     }
@@ -144,25 +155,35 @@ struct WarpState {
     float o[NT][HD / 16][4];
     float m[NT][2], l[NT][2], wmax[NT][2], gain[NT][2], factor[NT][2];
 
-    __device__ __forceinline__ void page(const PageRegs<HD>& r, float ks, float vs, int valid, int g, int c) {
-        float s[NT][4];
+    // Scores of one page; two sums side by side halve the chain of products.
+    __device__ __forceinline__ void scores(const KeyRegs<HD>& k, float (&s)[NT][4]) {
+        float s2[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[n][i] = 0.0f;
+            for (int i = 0; i < 4; i++) s[n][i] = s2[n][i] = 0.0f;
 #pragma unroll
         for (int j = 0; j < HD / 64; j++)
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 uint32_t a0, a1, a2, a3;
-                word_f16(r.k[0][j][w], a0, a2);
-                word_f16(r.k[1][j][w], a1, a3);
+                word_f16(k.w[0][j][w], a0, a2);
+                word_f16(k.w[1][j][w], a1, a3);
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    mma_f16(s[n], a0, a1, a2, a3, q[0][n][j][2 * w], q[0][n][j][2 * w + 1]);
-                    if constexpr (SPLIT) mma_f16(s[n], a0, a1, a2, a3, q[1][n][j][2 * w], q[1][n][j][2 * w + 1]);
+                    mma_f16((w & 1) && !SPLIT ? s2[n] : s[n], a0, a1, a2, a3, q[0][n][j][2 * w], q[0][n][j][2 * w + 1]);
+                    if constexpr (SPLIT) mma_f16(s2[n], a0, a1, a2, a3, q[1][n][j][2 * w], q[1][n][j][2 * w + 1]);
                 }
             }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[n][i] += s2[n][i];
+    }
+
+    // Scores to weights, as the second product's operand.
+    __device__ __forceinline__ void weights(float (&s)[NT][4], float ks, float vs, int valid, int g,
+                                            uint32_t (&b)[SPLIT ? 2 : 1][NT][2]) {
         bool moves = false;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -200,7 +221,6 @@ struct WarpState {
                     gain[n][h] = next;
                 }
         }
-        uint32_t b[SPLIT ? 2 : 1][NT][2];
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             float w[4];
@@ -217,11 +237,14 @@ struct WarpState {
                 if constexpr (SPLIT) b[1][n][i] = transpose8(pack_f16_rest(w[2 * i], w[2 * i + 1], hi));
             }
         }
+    }
+
+    __device__ __forceinline__ void add_values(const ValueRegs<HD>& r, const uint32_t (&b)[SPLIT ? 2 : 1][NT][2], int valid, int c) {
 #pragma unroll
         for (int i = 0; i < HD / 16; i++) {
             // bytes 2i, 2i + 1 of the lane's 4 rows: adjacent tokens' values of a dim side by side
             const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
-            uint32_t v0 = r.v[0][i / 2], v1 = r.v[1][i / 2], v2 = r.v[2][i / 2], v3 = r.v[3][i / 2];
+            uint32_t v0 = r.w[0][i / 2], v1 = r.w[1][i / 2], v2 = r.w[2][i / 2], v3 = r.w[3][i / 2];
             if (valid < kPage) {  // what lies behind the last token may be NaN
                 if (2 * c >= valid) v0 = 0;
                 if (2 * c + 1 >= valid) v1 = 0;
@@ -243,13 +266,17 @@ struct WarpState {
 __device__ __forceinline__ int context_of(const Kv8DecodeArgs& a, int b, bool& bad) {
     const int64_t n = a.ctx_lens[b], cap = (int64_t)a.max_pages * kPage;
     bad = n < 0 || n > cap;
-    return (int)((n < 0 ? 0 : n > cap ? cap : n) + kPage - 1) / kPage;
+    return (int)(((n < 0 ? 0 : n > cap ? cap : n) + kPage - 1) / kPage);
 }
 
 // exp2(m - top), for a part without tokens 0 (or its NaN).
 __device__ __forceinline__ float part_weight(float m, float top, float l) {
     return m == -INFINITY ? (l != l ? l : 0.0f) : exp2_fast(m - top);
 }
+
+// CTAs on an SM, by the registers a warp's state takes.
+template <typename T, int HD, int NT>
+constexpr int kCtas = NT == 2 ? (HD == 128 ? 2 : 3) : (HD == 128 && sizeof(T) == 4 ? 3 : 4);
 
 // Floats of a unit's partial result: group rows of HD values, then the group's maxima and
 // sums, a whole number of 16-byte pieces.
@@ -258,7 +285,7 @@ __host__ __device__ __forceinline__ int64_t partial_floats(int group, int head_d
 }
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kWarps * 32, HD * NT == 256 ? 2 : 3) kv8_decode_kernel(Kv8DecodeArgs a, float* partial, int* counters) {
+__global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kernel(Kv8DecodeArgs a, float* partial, int* counters) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int HEADS = 8 * NT, LD = HD + 4;
     __shared__ __align__(16) float s_o[kWarps][HEADS][LD], s_m[kWarps][HEADS], s_l[kWarps][HEADS];
@@ -279,15 +306,18 @@ __global__ void __launch_bounds__(kWarps * 32, HD * NT == 256 ? 2 : 3) kv8_decod
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
     if (blockIdx.x == 0 && any_bad) flag_error(a.err, kErrBadContext);
-    const int64_t per = (total * nkv + kUnits - 1) / kUnits;
-    const int chunk = (int64_t)a.B * nkv > kCounters ? INT32_MAX : (int)max((int64_t)kMinPages, min(per, (int64_t)INT32_MAX));
+    const int64_t items = (int64_t)a.B * nkv;
+    const int wanted = units_wanted(items, kSms * kCtas<T, HD, NT>);
+    const int64_t all = total * nkv;
+    const int per = all <= INT32_MAX - wanted ? ((int)all + wanted - 1) / wanted : (int)min((all + wanted - 1) / wanted, (int64_t)INT32_MAX);
+    const int chunk = items > kCounters ? INT32_MAX : max(kMinPages, per);
     const int unit = blockIdx.x;
     int b = -1, pages = 0, units = 0, at = 0;  // at: first unit of sequence b
     for (int i0 = 0, before = 0; i0 < a.B && b < 0; i0 += 32) {
         const int i = i0 + lane;
         bool bad;
         const int n = i < a.B ? context_of(a, i, bad) : 0;
-        const int u = i < a.B ? max(1, (int)(((int64_t)n + chunk - 1) / chunk)) : 0;  // an empty row is written too
+        const int u = i < a.B ? max(0, n - 1) / chunk + 1 : 0;  // an empty row is written too
         int sum = u;
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -310,6 +340,37 @@ __global__ void __launch_bounds__(kWarps * 32, HD * NT == 256 ? 2 : 3) kv8_decod
     const int pg0 = part * each, pg1 = min(pages, pg0 + each);
     const int ctx = min(max(a.ctx_lens[b], 0), pages * kPage);
 
+    // this warp's pages, 32 at a time: lane i looks up the i-th one's block and scales
+    const int mine = pg1 - pg0 > warp ? (pg1 - pg0 - warp + kWarps - 1) / kWarps : 0;
+    struct Lookup {
+        int64_t block;
+        float ks, vs;
+    };
+    auto look_up = [&](int base) {
+        Lookup x{-1, 0.0f, 0.0f};
+        if (base + lane < mine) {
+            const int pg = pg0 + warp + kWarps * (base + lane);
+            const int id = a.block_tables[(int64_t)b * a.max_pages + pg];
+            if (id >= 0 && id < a.pool.n_pages) {
+                x.block = ((int64_t)id * a.pool.n_layers + a.layer) * nkv + kvh;
+                x.ks = a.pool.k_scale[x.block];
+                x.vs = a.pool.v_scale[x.block];
+            } else {
+                flag_error(a.err, kErrBadContext);
+            }
+        }
+        return x;
+    };
+    Lookup now = look_up(0), next{-1, 0.0f, 0.0f};
+    KeyRegs<HD> kr;
+    ValueRegs<HD> vr;
+    int64_t block = __shfl_sync(0xffffffffu, now.block, 0);
+    if (block >= 0) {
+        kr.load(a.pool.k + block * (kPage * HD), g, c);
+        vr.load(a.pool.v + block * (kPage * HD), g, c);
+    }
+
+    // the queries, while the first page is on its way
     WarpState<HD, NT, SPLIT> st;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
@@ -359,43 +420,23 @@ __global__ void __launch_bounds__(kWarps * 32, HD * NT == 256 ? 2 : 3) kv8_decod
             for (int k = 0; k < 4; k++) st.o[n][i][k] = 0.0f;
     }
 
-    // this warp's pages, 32 at a time: lane i looks up the i-th one's block and scales
-    const int mine = pg1 - pg0 > warp ? (pg1 - pg0 - warp + kWarps - 1) / kWarps : 0;
-    for (int base = 0; base < mine; base += 32) {
-        const int count = min(32, mine - base);
-        int64_t block = -1;
-        float ks = 0.0f, vs = 0.0f;
-        if (lane < count) {
-            const int pg = pg0 + warp + kWarps * (base + lane);
-            const int id = a.block_tables[(int64_t)b * a.max_pages + pg];
-            if (id >= 0 && id < a.pool.n_pages) {
-                block = ((int64_t)id * a.pool.n_layers + a.layer) * nkv + kvh;
-                ks = a.pool.k_scale[block];
-                vs = a.pool.v_scale[block];
-            } else {
-                flag_error(a.err, kErrBadContext);
-            }
+    // A page's keys are replaced by the next page's as soon as they are used, its values too.
+    for (int i = 0; i < mine; i++) {
+        if (i % 32 == 0) next = look_up(i + 32);
+        const float ks = __shfl_sync(0xffffffffu, now.ks, i % 32), vs = __shfl_sync(0xffffffffu, now.vs, i % 32);
+        if (i % 32 == 31) now = next;
+        const int64_t following = __shfl_sync(0xffffffffu, now.block, (i + 1) % 32);  // -1 behind the last
+        const int left = ctx - (pg0 + warp + kWarps * i) * kPage;
+        float s[NT][4];
+        uint32_t w[SPLIT ? 2 : 1][NT][2];
+        if (block >= 0) st.scores(kr, s);
+        if (following >= 0) kr.load(a.pool.k + following * (kPage * HD), g, c);
+        if (block >= 0) {
+            st.weights(s, ks, vs, left, g, w);
+            st.add_values(vr, w, left, c);
         }
-        PageRegs<HD> r[2];
-        auto fetch = [&](PageRegs<HD>& x, int i) {
-            const int64_t blk = __shfl_sync(0xffffffffu, block, i);
-            if (blk >= 0) x.load(a.pool.k + blk * (kPage * HD), a.pool.v + blk * (kPage * HD), g, c);
-        };
-        auto use = [&](const PageRegs<HD>& x, int i) {
-            const int64_t blk = __shfl_sync(0xffffffffu, block, i);
-            const float kk = __shfl_sync(0xffffffffu, ks, i), vv = __shfl_sync(0xffffffffu, vs, i);
-            const int left = ctx - (pg0 + warp + kWarps * (base + i)) * kPage;
-            if (blk >= 0) st.page(x, kk, vv, left, g, c);
-        };
-        fetch(r[0], 0);
-        for (int i = 0; i < count; i += 2) {
-            if (i + 1 < count) fetch(r[1], i + 1);
-            use(r[0], i);
-            if (i + 1 < count) {
-                if (i + 2 < count) fetch(r[0], i + 2);
-                use(r[1], i + 1);
-            }
-        }
+        if (following >= 0) vr.load(a.pool.v + following * (kPage * HD), g, c);
+        block = following;
     }
 
     // join the warps
@@ -441,49 +482,72 @@ __global__ void __launch_bounds__(kWarps * 32, HD * NT == 256 ? 2 : 3) kv8_decod
         }
     }
     if (units == 1) return;
-    __threadfence();
     __syncthreads();
     if (threadIdx.x == 0) {
+        // release: what the CTA wrote before the barrier; acquire: what the others did
         int* n = counters + b * nkv + kvh;
-        const int before = atomicAdd(n, 1);
+        int before;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(n) : "memory");
         s_last = before == units - 1;
         if (s_last) *n = 0;
     }
     __syncthreads();
     if (!s_last) return;
-    __threadfence();
+    // the weights of the parts: a warp for each head, a lane for each part
     const float* first = partial + ((int64_t)at * nkv + kvh) * rec;
     const int64_t step = (int64_t)nkv * rec;
+    for (int head = warp; head < group; head += kWarps) {
+        float top = -INFINITY;
+        for (int u = lane; u < units; u += 32) top = fmaxf(top, __ldcg(first + u * step + group * HD + head));
+        top = warp_max(top);
+        float l = 0.0f;
+        for (int u = lane; u < units; u += 32) {
+            const float pl = __ldcg(first + u * step + group * HD + group + head);
+            l += part_weight(__ldcg(first + u * step + group * HD + head), top, pl) * pl;
+        }
+        l = warp_sum(l);
+        if (lane == 0) s_m[0][head] = top, s_l[0][head] = l == 0.0f ? 0.0f : 1.0f / l;
+    }
+    __syncthreads();
     for (int e = threadIdx.x * 4; e < group * HD; e += blockDim.x * 4) {
         const int head = e / HD;
-        float top = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-        for (int u = 0; u < units; u++) top = fmaxf(top, __ldcg(first + u * step + group * HD + head));
-#pragma unroll 4
-        for (int u = 0; u < units; u++) {
-            const float* p = first + u * step;
-            const float pl = __ldcg(p + group * HD + group + head);
-            const float f = part_weight(__ldcg(p + group * HD + head), top, pl);
-            l += f * pl;
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + e));
-            acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
+        const float top = s_m[0][head], inv = s_l[0][head];
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u0 = 0; u0 < units; u0 += 8) {
+            float4 v[8];
+            float m[8], l[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float* p = first + min(u0 + i, units - 1) * step;
+                v[i] = __ldcg(reinterpret_cast<const float4*>(p + e));
+                m[i] = __ldcg(p + group * HD + head);
+                l[i] = __ldcg(p + group * HD + group + head);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float f = u0 + i < units ? part_weight(m[i], top, l[i]) : 0.0f;
+                if (f != 0.0f) {
+                    acc[0] += f * v[i].x; acc[1] += f * v[i].y; acc[2] += f * v[i].z; acc[3] += f * v[i].w;
+                }
+            }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int i = 0; i < 4; i++) out[e + i] = from_f32<T>(acc[i] * inv);
     }
 }
 
-int64_t most_units(int B, int n_kv_heads) { return (int64_t)B * n_kv_heads + kUnits; }
+template <typename T, int HD, int NT>
+cudaError_t launch_nt(const Kv8DecodeArgs& a, cudaStream_t s) {
+    int* counters = (int*)a.workspace;
+    float* partial = (float*)((char*)a.workspace + kCounters * sizeof(int));
+    const int64_t items = (int64_t)a.B * a.pool.n_kv_heads;
+    const dim3 grid((unsigned)(items + units_wanted(items, kSms * kCtas<T, HD, NT>)));
+    return launch_ex(kv8_decode_kernel<T, HD, NT>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters);
+}
 
 template <typename T, int HD>
 cudaError_t launch_hd(const Kv8DecodeArgs& a, cudaStream_t s) {
-    int* counters = (int*)a.workspace;
-    float* partial = (float*)((char*)a.workspace + kCounters * sizeof(int));
-    const dim3 grid((unsigned)most_units(a.B, a.pool.n_kv_heads));
-    if (a.n_heads / a.pool.n_kv_heads <= 8)
-        return launch_ex(kv8_decode_kernel<T, HD, 1>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters);
-    return launch_ex(kv8_decode_kernel<T, HD, 2>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters);
+    return a.n_heads / a.pool.n_kv_heads <= 8 ? launch_nt<T, HD, 1>(a, s) : launch_nt<T, HD, 2>(a, s);
 }
 
 template <typename T>
@@ -495,7 +559,8 @@ cudaError_t launch_t(const Kv8DecodeArgs& a, cudaStream_t s) {
 
 size_t kv8_decode_workspace_bytes(int B, int n_heads, int n_kv_heads, int head_dim, int) {
     const size_t rec = partial_floats(n_heads / n_kv_heads, head_dim) * sizeof(float);
-    const size_t n = (int64_t)B * n_kv_heads > kCounters ? 0 : (size_t)most_units(B, n_kv_heads) * rec;
+    const int64_t items = (int64_t)B * n_kv_heads;
+    const size_t n = items > kCounters ? 0 : (size_t)(items + kWaves * kSms * kMostCtas) * rec;
     return kCounters * sizeof(int) + (n + 255) / 256 * 256;
 }
 
