@@ -41,15 +41,18 @@ namespace nitro {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kWaves = 4;
-constexpr int kSms = 148, kMostCtas = 4;
+constexpr int kWaves = 2;
+constexpr int kSms = 148, kMostCtas = 5;
 // Pages are cut into so many units, `slots` of which run at once.  With few items the last
 // units should not start a second wave (each item can add one unit to the even cut); many
 // items run in several waves anyway, which smaller units even out.
 __host__ __device__ __forceinline__ int units_wanted(int64_t items, int slots) {
     return items <= slots / 2 ? slots - (int)items : kWaves * slots;
 }
-constexpr int kMinPages = 8;            // of a unit: two for each warp
+// A unit's least pages: two for each warp where units are few, more where there are enough
+// items to fill the device (64 sequences of 128..1024 tokens, 12 kv heads: 31 us with units
+// of 16 pages and up, 26.6 with 64).
+constexpr int kMinPages = 8, kMinPagesMany = 64;
 // Items whose partial results can be counted; more items than that fill the device uncut.
 constexpr int kCounters = 16384;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -276,7 +279,7 @@ __device__ __forceinline__ float part_weight(float m, float top, float l) {
 
 // CTAs on an SM, by the registers a warp's state takes.
 template <typename T, int HD, int NT>
-constexpr int kCtas = NT == 2 ? (HD == 128 ? 2 : 3) : (HD == 128 && sizeof(T) == 4 ? 3 : 4);
+constexpr int kCtas = NT == 2 ? (HD == 128 ? 2 : 3) : HD == 64 ? 5 : sizeof(T) == 4 ? 3 : 4;
 
 // Floats of a unit's partial result: group rows of HD values, then the group's maxima and
 // sums, a whole number of 16-byte pieces.
@@ -295,28 +298,35 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kern
     grid_dependency_wait();
     grid_dependents_launch();
 
-    // the cut: all pages over kUnits, then the sequence this unit belongs to
+    // the cut: all pages over the units wanted, then the sequence this unit belongs to
     int64_t total = 0;
     bool any_bad = false;
+    int first_n = 0;  // pages of sequence `lane`
     for (int i = lane; i < a.B; i += 32) {
         bool bad;
-        total += context_of(a, i, bad);
+        const int n = context_of(a, i, bad);
+        if (i == lane) first_n = n;
+        total += n;
         any_bad |= bad;
     }
+    if (a.B <= 32) {  // at most 2^31 together: one number to a lane
+        total = __reduce_add_sync(0xffffffffu, (uint32_t)total);
+    } else {
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+        for (int x = 16; x > 0; x >>= 1) total += __shfl_xor_sync(0xffffffffu, total, x);
+    }
     if (blockIdx.x == 0 && any_bad) flag_error(a.err, kErrBadContext);
     const int64_t items = (int64_t)a.B * nkv;
     const int wanted = units_wanted(items, kSms * kCtas<T, HD, NT>);
     const int64_t all = total * nkv;
     const int per = all <= INT32_MAX - wanted ? ((int)all + wanted - 1) / wanted : (int)min((all + wanted - 1) / wanted, (int64_t)INT32_MAX);
-    const int chunk = items > kCounters ? INT32_MAX : max(kMinPages, per);
+    const int chunk = items > kCounters ? INT32_MAX : max(items <= kSms ? kMinPages : kMinPagesMany, per);
     const int unit = blockIdx.x;
     int b = -1, pages = 0, units = 0, at = 0;  // at: first unit of sequence b
     for (int i0 = 0, before = 0; i0 < a.B && b < 0; i0 += 32) {
         const int i = i0 + lane;
         bool bad;
-        const int n = i < a.B ? context_of(a, i, bad) : 0;
+        const int n = i0 == 0 ? first_n : i < a.B ? context_of(a, i, bad) : 0;
         const int u = i < a.B ? max(0, n - 1) / chunk + 1 : 0;  // an empty row is written too
         int sum = u;
 #pragma unroll
