@@ -245,6 +245,15 @@ int nr_replay_decode_attention(nr_engine* e, int32_t n, int32_t with_merge);
  * [B]) the greedy ids, logits_out (if not NULL, [B x vocab]) the logits, which only a step
  * that computed them has (NR_ERR_INVALID otherwise).  Synchronises the engine stream. */
 int nr_decode_last_outputs(nr_engine* e, int32_t* argmax_out, float* logits_out, int32_t* B_out);
+/* Log probabilities of the most recent decode step or replay that computed logits
+ * (NR_ERR_INVALID otherwise), taken on the GPU from the logits still there: *B_out rows;
+ * target_logprob[b] of the token targets[b] (both NULL, or NaN for an id outside the
+ * vocabulary), entropy[b] in nats (may be NULL), and the top_k (<= NR_LOGPROBS_MAX_TOP,
+ * defined below) largest ids and log probabilities, row by row.  Statistics as
+ * nr_token_logprobs.  No counterpart in the reference, which has the greedy id only.
+ * Synchronises the engine stream. */
+int nr_decode_last_logprobs(nr_engine* e, const int32_t* targets, int32_t top_k, float* target_logprob,
+                            float* entropy, float* top_logprob, int32_t* top_ids, int32_t* B_out);
 
 typedef struct nr_stats {
     int64_t steps, prefill_tokens, decode_tokens, cache_hit_pages, evictions, kernel_launches;

@@ -609,6 +609,14 @@ int nr_decode_last_outputs(nr_engine* e, int32_t* argmax_out, float* logits_out,
     return e->impl->last_decode_outputs(argmax_out, logits_out, B_out);
 }
 
+int nr_decode_last_logprobs(nr_engine* e, const int32_t* targets, int32_t top_k, float* target_logprob, float* entropy,
+                            float* top_logprob, int32_t* top_ids, int32_t* B_out) {
+    if (!e || top_k < 0 || top_k > NR_LOGPROBS_MAX_TOP || top_k > e->impl->shape().vocab) return NR_ERR_INVALID;
+    if (!targets != !target_logprob || (top_k ? !top_logprob || !top_ids : top_logprob || top_ids)) return NR_ERR_INVALID;
+    if (!targets && !entropy && !top_k) return NR_ERR_INVALID;
+    return e->impl->last_decode_logprobs(targets, top_k, target_logprob, entropy, top_logprob, top_ids, B_out);
+}
+
 int nr_engine_stats(nr_engine* e, nr_stats* out) {
     if (!e || !out) return NR_ERR_INVALID;
     *out = e->impl->stats;

@@ -17,6 +17,7 @@
 #include <string>
 
 #include "engine.h"
+#include "kv8.h"
 
 namespace nitro {
 
@@ -84,6 +85,7 @@ Engine::~Engine() {
     cudaFree(d_att_);
     cudaFree(d_h_);
     cudaFree(d_logits_);
+    cudaFree(d_scores_);
     cudaFree(d_keys_);
     cudaFree(d_ss_);
     cudaFree(d_xs_);
@@ -800,6 +802,41 @@ int Engine::last_decode_outputs(int* argmax_out, float* logits_out, int* B_out) 
     NR_CUDA(cudaStreamSynchronize(stream_));
     if (h_argmax_[0] != 0) return fail(NR_ERR_TIMEOUT, "device wait timed out");
     if (argmax_out) memcpy(argmax_out, h_argmax_ + 1, (size_t)last_B_ * 4);
+    if (B_out) *B_out = last_B_;
+    return NR_OK;
+}
+
+int Engine::last_decode_logprobs(const int* targets, int top_k, float* target_logprob, float* entropy, float* top_logprob,
+                                 int* top_ids, int* B_out) {
+    if (!has_device()) return fail(NR_ERR_NO_DEVICE, "host-only engine");
+    if (!last_valid_) return fail(NR_ERR_INVALID, "no decode step ran");
+    if (!last_logits_) return fail(NR_ERR_INVALID, "the last decode step computed no logits");
+    NR_CUDA(cudaSetDevice(cfg_.device));
+    // [targets | target_logprob | entropy | top_logprob | top_ids], made on the first call
+    const size_t R = cfg_.max_batch, K = NR_LOGPROBS_MAX_TOP;
+    if (!d_scores_) NR_CUDA(cudaMalloc(&d_scores_, R * (3 + 2 * K) * 4));
+    const size_t B = last_B_;
+    LogprobArgs a;
+    int* d_targets = (int*)d_scores_;
+    a.logits = d_logits_; a.dtype = kF32; a.row_stride = shape_.vocab; a.M = last_B_; a.V = shape_.vocab; a.top_k = top_k;
+    a.target_logprob = targets ? d_scores_ + R : nullptr;
+    a.entropy = entropy ? d_scores_ + 2 * R : nullptr;
+    a.top_logprob = d_scores_ + 3 * R;
+    a.top_ids = (int*)(d_scores_ + (3 + K) * R);
+    if (targets) {
+        NR_CUDA(cudaMemcpyAsync(d_targets, targets, B * 4, cudaMemcpyHostToDevice, stream_));
+        a.targets = d_targets;
+    }
+    NR_CUDA(cudaMemcpyAsync(h_argmax_, d_err_, 4, cudaMemcpyDeviceToHost, stream_));
+    NR_CUDA(launch_token_logprobs(a, stream_));
+    if (targets) NR_CUDA(cudaMemcpyAsync(target_logprob, a.target_logprob, B * 4, cudaMemcpyDeviceToHost, stream_));
+    if (entropy) NR_CUDA(cudaMemcpyAsync(entropy, a.entropy, B * 4, cudaMemcpyDeviceToHost, stream_));
+    if (top_k) {
+        NR_CUDA(cudaMemcpyAsync(top_logprob, a.top_logprob, B * top_k * 4, cudaMemcpyDeviceToHost, stream_));
+        NR_CUDA(cudaMemcpyAsync(top_ids, a.top_ids, B * top_k * 4, cudaMemcpyDeviceToHost, stream_));
+    }
+    NR_CUDA(cudaStreamSynchronize(stream_));
+    if (h_argmax_[0] != 0) return fail(NR_ERR_TIMEOUT, "device wait timed out");
     if (B_out) *B_out = last_B_;
     return NR_OK;
 }

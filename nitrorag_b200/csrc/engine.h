@@ -111,6 +111,8 @@ public:
     // Outputs of the most recent decode step or replay: B argmax ids, and the B x vocab
     // logits when that step computed them (synchronises the engine stream).
     int last_decode_outputs(int* argmax_out, float* logits_out, int* B_out);
+    int last_decode_logprobs(const int* targets, int top_k, float* target_logprob, float* entropy, float* top_logprob,
+                             int* top_ids, int* B_out);
 
     // profiling: CUDA events around every launch, accumulated per KernelClass
     int set_profiling(bool on);
@@ -153,6 +155,7 @@ private:
     float* d_att_ = nullptr;   // [max_rows][dim]
     float* d_h_ = nullptr;     // [max_rows][hidden]
     float* d_logits_ = nullptr;  // [max_batch][vocab]
+    float* d_scores_ = nullptr;  // log probabilities of the last step, made on first use
     unsigned long long* d_keys_ = nullptr;  // [max_rows]
     float* d_ss_ = nullptr;    // [ceil(dim/128)][max_rows] partial sums of squares of x
     int* d_argmax_ = nullptr;  // [max_rows]

@@ -167,6 +167,36 @@ class NitroEngine:
         self._check(lib().nr_decode_last_outputs(self._h, _pi32(am), _pf(lg), C.byref(B)), "nr_decode_last_outputs")
         return am[:B.value].copy(), (None if lg is None else lg[:B.value].copy())
 
+    def last_decode_logprobs(self, targets=None, top_k: int = 0) -> dict:
+        """Log probabilities of the most recent decode step that computed logits, taken on the
+        GPU: "entropy" [B], with ``targets`` (one token id per row) "target" [B], with
+        ``top_k`` "top_ids" and "top" [B][top_k], largest first."""
+        cap = self.config.max_batch
+        t = None
+        if targets is not None:
+            t = np.zeros(cap, np.int32)
+            given = _i32(targets)
+            if len(given) > cap:
+                raise NrError(-8, "nr_decode_last_logprobs", "more targets than max_batch")
+            t[:len(given)] = given
+        tl = None if t is None else np.zeros(cap, np.float32)
+        en = np.zeros(cap, np.float32)
+        tp = np.zeros((cap, max(top_k, 0)), np.float32)
+        ids = np.zeros((cap, max(top_k, 0)), np.int32)
+        B = C.c_int32(0)
+        self._check(lib().nr_decode_last_logprobs(
+            self._h, None if t is None else _pi32(t), top_k, _pf(tl), _pf(en), _pf(tp) if top_k else None,
+            _pi32(ids) if top_k else None, C.byref(B)), "nr_decode_last_logprobs")
+        n = B.value
+        if t is not None and len(given) != n:
+            raise NrError(-1, "nr_decode_last_logprobs", f"{len(given)} targets for {n} rows")
+        out = dict(entropy=en[:n].copy())
+        if t is not None:
+            out["target"] = tl[:n].copy()
+        if top_k:
+            out["top_ids"], out["top"] = ids[:n].copy(), tp[:n].copy()
+        return out
+
     # ------------------------------------------------------------ scheduler
     def add_request(self, req_id: int, prompt) -> None:
         p = _i32(prompt)

@@ -115,3 +115,18 @@ def test_every_unit_of_packed_rows_is_covered():
                 pieces = (start + m - 1) // W - start // W + 1 if m else 0
                 room = cu[b + 1] // W + n * (b + 1) - (cu[b] // W + n * b)
                 assert pieces <= room
+
+
+def test_engine_logprobs_without_gpu():
+    from nitrorag_b200 import EngineConfig, NitroEngine, NrError
+    eng = NitroEngine(config=EngineConfig(total_blocks=8, device=-1), shape=(64, 128, 2, 2, 2, 100, 64))
+    with pytest.raises(NrError, match="NO_DEVICE"):
+        eng.last_decode_logprobs(top_k=1)
+    f, i = (C.c_float * 8)(), (C.c_int32 * 8)()
+    call = lib().nr_decode_last_logprobs
+    for args in ((None, -1, None, f, None, None, None), (None, 33, None, f, f, i, None), (None, 0, None, None, None, None, None),
+                 (i, 0, None, f, None, None, None), (None, 0, f, f, None, None, None), (None, 1, None, f, None, i, None),
+                 (None, 0, None, f, f, i, None)):
+        assert call(eng._h, *args) == INVALID
+    assert call(None, None, 0, None, f, None, None, None) == INVALID
+    eng.close()
