@@ -680,6 +680,13 @@ static bool read_kv8_pool(const nr_kv8_pool* p, int32_t layer, nitro::Kv8Pool* o
     return true;
 }
 
+// A failed launch's error is not left for the next call that asks for the last one.
+static int launched(cudaError_t rc) {
+    if (rc == cudaSuccess) return NR_OK;
+    cudaGetLastError();
+    return NR_ERR_CUDA;
+}
+
 static bool valid_dtype(int32_t dtype) { return dtype == NR_DTYPE_F32 || dtype == NR_DTYPE_BF16 || dtype == NR_DTYPE_F16; }
 
 // Rows of `width` elements at a stride that keeps each row 16-byte aligned.
@@ -690,7 +697,7 @@ static bool valid_rows(const void* p, int64_t stride, int64_t width, int32_t dty
 int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* g, int32_t* error_flag, void* stream) {
     nitro::Kv8AppendArgs a;
     if (!g || !read_kv8_pool(pool, g->layer, &a.pool) || !valid_dtype(g->dtype)) return NR_ERR_INVALID;
-    if (!g->cu_seqlens || !g->start_pos || !g->block_tables || g->B <= 0 || g->B > 1024 || g->T <= 0 || g->max_pages <= 0)
+    if (!g->cu_seqlens || !g->start_pos || !g->block_tables || g->B <= 0 || g->B > 1024 || g->T <= 0 || g->T > (1 << 30) || g->max_pages <= 0)
         return NR_ERR_INVALID;
     const int hd = pool->head_dim;
     const int64_t kw = (int64_t)pool->n_kv_heads * hd, qw = (int64_t)g->n_heads * hd;
@@ -715,7 +722,7 @@ int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* g, int32_t*
     a.rope_cos = g->rope_cos; a.rope_sin = g->rope_sin;
     a.dtype = g->dtype; a.B = g->B; a.T = g->T; a.n_heads = g->n_heads; a.max_pages = g->max_pages; a.layer = g->layer;
     a.rope_len = g->rope_len; a.rot_dim = g->rot_dim; a.rope_layout = g->rope_layout; a.err = error_flag;
-    return nitro::launch_kv8_append(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+    return launched(nitro::launch_kv8_append(a, (cudaStream_t)stream));
 }
 
 size_t nr_paged_attention_kv8_workspace_size(int32_t B, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
@@ -735,7 +742,7 @@ int nr_paged_attention_decode_kv8(const void* q, int32_t dtype, const nr_kv8_poo
     if (!nr_paged_attention_kv8_workspace_size(B, n_heads, pool->n_kv_heads, pool->head_dim, max_pages)) return NR_ERR_INVALID;
     a.q = q; a.out = out; a.block_tables = block_tables; a.ctx_lens = ctx_lens; a.workspace = workspace;
     a.dtype = dtype; a.layer = layer; a.max_pages = max_pages; a.B = B; a.n_heads = n_heads; a.err = error_flag;
-    return nitro::launch_kv8_decode(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+    return launched(nitro::launch_kv8_decode(a, (cudaStream_t)stream));
 }
 
 int nr_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
@@ -744,6 +751,7 @@ int nr_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t 
                         int32_t head_dim, int32_t* error_flag, void* stream) {
     if (dtype != NR_DTYPE_BF16 && dtype != NR_DTYPE_F16) return NR_ERR_INVALID;
     if (!cu_q || B <= 0 || B > 1024 || Tq <= 0 || Tk <= 0 || (!cu_k && Tq != Tk)) return NR_ERR_INVALID;
+    if (Tq > (1 << 30) || Tk > (1 << 30)) return NR_ERR_INVALID;
     if (n_heads <= 0 || n_heads > (1 << 15) || n_kv_heads <= 0 || n_heads % n_kv_heads) return NR_ERR_INVALID;
     if (head_dim != 64 && head_dim != 128) return NR_ERR_INVALID;
     const int64_t qw = (int64_t)n_heads * head_dim, kw = (int64_t)n_kv_heads * head_dim;
@@ -754,7 +762,7 @@ int nr_prompt_attention(const void* q, int64_t q_stride, const void* k, int64_t 
     a.q = q; a.k = k; a.v = v; a.out = out; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
     a.out_stride = out_stride; a.cu_q = cu_q; a.cu_k = cu_k; a.dtype = dtype; a.B = B; a.Tq = Tq; a.Tk = Tk;
     a.n_heads = n_heads; a.n_kv_heads = n_kv_heads; a.head_dim = head_dim; a.err = error_flag;
-    return nitro::launch_prompt_attention(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+    return launched(nitro::launch_prompt_attention(a, (cudaStream_t)stream));
 }
 
 int nr_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int32_t M, int32_t V,
@@ -769,7 +777,7 @@ int nr_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, int
     a.logits = logits; a.dtype = dtype; a.row_stride = row_stride; a.M = M; a.V = V; a.top_k = top_k;
     a.targets = targets; a.target_logprob = target_logprob; a.entropy = entropy; a.top_logprob = top_logprob;
     a.top_ids = top_ids;
-    return nitro::launch_token_logprobs(a, (cudaStream_t)stream) == cudaSuccess ? NR_OK : NR_ERR_CUDA;
+    return launched(nitro::launch_token_logprobs(a, (cudaStream_t)stream));
 }
 
 size_t nr_q8_quantized_size(int64_t n) { return nitro::q8_quantized_bytes(n); }

@@ -231,16 +231,20 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_append_kernel(Kv8Appen
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     grid_dependency_wait();
     grid_dependents_launch();
+    auto in_range = [&](int r0, int r1, int at) {
+        const int64_t end = (int64_t)at + r1 - r0;
+        return r0 >= 0 && r1 >= r0 && r1 <= a.T && at >= 0 && end <= (int64_t)a.max_pages * kPage && (ROT == kNone || end <= a.rope_len);
+    };
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = threadIdx.x; i < a.B; i += blockDim.x)
+            if (a.cu_seqlens[i] != a.cu_seqlens[i + 1] && !in_range(a.cu_seqlens[i], a.cu_seqlens[i + 1], a.start_pos[i]))
+                flag_error(a.err, kErrBadContext);
     const int b = seq_of_unit<kPage, 2>(a.cu_seqlens, a.B, blockIdx.x, lane);
     const int row0 = a.cu_seqlens[b], row1 = a.cu_seqlens[b + 1], start = a.start_pos[b];
     const int j = (int)blockIdx.x - (row0 / kPage + 2 * b);
     if (j < 0 || row1 == row0) return;
     const int64_t end = (int64_t)start + row1 - row0;
-    if (row0 < 0 || row1 < row0 || row1 > a.T || start < 0 || end > (int64_t)a.max_pages * kPage ||
-        (ROT != kNone && end > a.rope_len)) {
-        if (j == 0 && threadIdx.x == 0) flag_error(a.err, kErrBadContext);
-        return;
-    }
+    if (!in_range(row0, row1, start)) return;
     const int pg = start / kPage + j;
     if ((int64_t)pg * kPage >= end) return;
     const int pos0 = max(start, pg * kPage);
@@ -284,6 +288,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) kv8_append_kernel(Kv8Appen
     }
 
     while (tile < tiles) {
+        __syncwarp();  // rows that repeat the last token are read before that is written in place
         if (tile < nq) {
             now.template turn<ROT, false>((T*)a.q_out + (int64_t)tile * HD, a.q_out_stride, u, s_cos, s_sin);
         } else if (tile < nq + nkv) {

@@ -216,15 +216,12 @@ __global__ void __launch_bounds__(Layout<HD, TILING>::kThreads, Layout<HD, TILIN
     extern __shared__ uint8_t smem_raw[];
     __shared__ Barriers bar;
     __shared__ uint32_t tmem_slot;
+    __shared__ int s_tile, s_q0, s_q1, s_k0, s_k1;
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint8_t* sq = smem;                                   // [tile][box]
     uint8_t* sk = sq + TILES * BOXES * kBox;              // [stage][box]
     uint8_t* sv = sk + kStages * BOXES * kBox;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == L::kMmaWarp) {
-        tmem_alloc(&tmem_slot, L::kTmem);
-        tmem_relinquish();
-    }
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
 #pragma unroll
@@ -246,24 +243,40 @@ __global__ void __launch_bounds__(Layout<HD, TILING>::kThreads, Layout<HD, TILIN
         fence_async_smem();
     }
     grid_dependency_wait();
-    grid_dependents_launch();
+    // Tensor memory is taken after the wait and before the next kernel may start: a CTA that
+    // holds some never waits for a kernel whose CTAs still want theirs.
+    if (warp == L::kMmaWarp) {
+        tmem_alloc(&tmem_slot, L::kTmem);
+        tmem_relinquish();
+    }
 
-    // heads of one tile side by side (they share keys in L2), later tiles (more keys) first
+
+    // heads of one tile side by side (they share keys in L2), later tiles (more keys) of a
+    // sequence first
     const int ny = TILING == kHeads ? a.n_heads / 2 : a.n_heads;
-    const int unit = n_units - 1 - (int)(blockIdx.x / ny);
     const int head0 = (int)(blockIdx.x % ny) * (TILING == kHeads ? 2 : 1);
     const int kvh = head0 / (a.n_heads / a.n_kv_heads);
     const int* cu_k = a.cu_k ? a.cu_k : a.cu_q;
-    const int b = seq_of_unit<W, 1>(a.cu_q, a.B, unit, lane);
-    const int q0 = a.cu_q[b], q1 = a.cu_q[b + 1], k0 = cu_k[b], k1 = cu_k[b + 1];
-    const int tile = unit - (q0 / W + b);
-    const bool fits = q0 >= 0 && q1 >= q0 && q1 <= a.Tq && k0 >= 0 && k1 >= k0 && k1 <= a.Tk;
-    if (!fits && q0 != q1 && tile == 0 && threadIdx.x == 0) flag_error(a.err, kErrBadContext);
+    auto usable = [&](int i) {
+        return a.cu_q[i] >= 0 && a.cu_q[i + 1] >= a.cu_q[i] && a.cu_q[i + 1] <= a.Tq && cu_k[i] >= 0 && cu_k[i + 1] >= cu_k[i] &&
+               cu_k[i + 1] <= a.Tk;
+    };
+    if (warp == L::kCopyWarp) {
+        const int unit = n_units - 1 - (int)(blockIdx.x / ny), b = seq_of_unit<W, 1>(a.cu_q, a.B, unit, lane);
+        const int q0 = a.cu_q[b], q1 = a.cu_q[b + 1], tile = unit - (q0 / W + b);
+        const bool any = usable(b) && tile >= 0 && (int64_t)tile * W < q1 - q0;
+        if (lane == 0) s_tile = any ? tile : -1, s_q0 = q0, s_q1 = q1, s_k0 = cu_k[b], s_k1 = cu_k[b + 1];
+    } else if (blockIdx.x == 0 && warp < L::kCopyWarp) {  // sequences that no CTA can work on
+        for (int i = threadIdx.x; i < a.B; i += 32 * L::kCopyWarp)
+            if (!usable(i)) flag_error(a.err, kErrBadContext);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    grid_dependents_launch();
     const uint32_t tmem = tmem_slot;
-    if (!fits || tile < 0 || (int64_t)tile * W >= q1 - q0) {  // nothing of a sequence
+    const int tile = s_tile, q0 = s_q0, q1 = s_q1, k0 = s_k0, k1 = s_k1;
+    if (tile < 0) {  // nothing of a sequence
         if (warp == L::kMmaWarp) tmem_dealloc(tmem, L::kTmem);
         return;
     }

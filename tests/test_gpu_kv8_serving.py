@@ -138,7 +138,7 @@ def test_engine_last_decode_logprobs(tiny_model):
         h = -(np.exp(lp) * lp).sum(-1)
         assert np.abs(got["entropy"] - h).max() <= 2.0 ** -18 * 12
         assert set(eng.last_decode_logprobs(top_k=0)) == {"entropy"}
-        lg2, _ = eng.last_decode_outputs(want_logits=True)
+        _, lg2 = eng.last_decode_outputs(want_logits=True)
         assert np.array_equal(lg, lg2)  # asking changed nothing
     with pytest.raises(NrError):
         eng.last_decode_logprobs(top_k=33)
