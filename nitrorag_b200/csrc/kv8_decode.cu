@@ -24,9 +24,20 @@
 // Work: the pages of all (sequence, kv head) items are cut into units of about equal
 // length, one CTA each, its four warps taking every fourth page.  The cut goes by the
 // lengths on the device, so a ragged batch and a table much wider than its contexts cost
-// nothing.  An item of one unit is finished by its CTA; otherwise the partial results go
-// to the workspace and the item's last CTA joins them in order (the result does not
-// depend on which CTA that is).
+// nothing.  An item of one unit is finished by its CTA.  The units of a longer one leave their
+// maximum, sum and output in the workspace, joined in order (the result does not depend on
+// who finishes last): up to kJoinItems items, each of many parts, by a second kernel with a
+// CTA for each head (2 sequences of 57k tokens, 16 heads on one: 87 -> 23 us; 4096 tokens, 8
+// items: 13.5 -> 10.2; but at 64 items 26.5 -> 27.0); else by the item's last CTA.
+//
+// Measured (of the copy bandwidth): 2 contexts of 131k tokens, 32 heads on 8, head_dim 128,
+// fp16: 104 us, 5.2 TB/s (0.79; the ALU, mostly the conversions of the codes, is at 46 %).  96
+// contexts of 0..4096 tokens, the same heads: 100 us, 4.2 TB/s (0.64): a page's scales and
+// codes are addressed by a table entry that has to be read first, and a unit's start and end
+// read nothing.  64 contexts of 128..1024, 12 heads of 64, fp32: 25 us, 2.3 TB/s (0.35), of
+// which about 8 us are a single unit's chain of latencies, as one context of 601 tokens takes.
+// Tried and left: runs of equal length over item borders, several items' pieces to a CTA
+// (27 -> 36, 100 -> 115 us: the pieces' latencies come one after another).
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
@@ -55,6 +66,7 @@ __host__ __device__ __forceinline__ int units_wanted(int64_t items, int slots) {
 constexpr int kMinPages = 8, kMinPagesMany = 64;
 // Items whose partial results can be counted; more items than that fill the device uncut.
 constexpr int kCounters = 16384;
+constexpr int kJoinItems = 32;  // most items whose parts a second kernel joins
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -288,7 +300,7 @@ __host__ __device__ __forceinline__ int64_t partial_floats(int group, int head_d
 }
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kernel(Kv8DecodeArgs a, float* partial, int* counters) {
+__global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kernel(Kv8DecodeArgs a, float* partial, int* counters, int2* items_cut) {
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int HEADS = 8 * NT, LD = HD + 4;
     __shared__ __align__(16) float s_o[kWarps][HEADS][LD], s_m[kWarps][HEADS], s_l[kWarps][HEADS];
@@ -491,6 +503,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kern
             if (d == 0) mine_out[group * HD + head] = top, mine_out[group * HD + group + head] = l;
         }
     }
+    if (items_cut) {
+        if (part == 0 && threadIdx.x == 0) items_cut[b * nkv + kvh] = make_int2(unit, units);
+        return;
+    }
     if (units == 1) return;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -546,13 +562,62 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kern
     }
 }
 
+// The parts of one head's item: `items_cut` has an item's first unit and how many it has.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) kv8_join_kernel(Kv8DecodeArgs a, const float* partial, const int2* items_cut) {
+    constexpr int LANES = HD / 4, SLICES = 128 / LANES;  // four dims to a thread, every SLICES-th part
+    __shared__ __align__(16) float s_o[SLICES][HD];
+    __shared__ float s_l[SLICES], s_top;
+    const int nkv = a.pool.n_kv_heads, group = a.n_heads / nkv;
+    const int b = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads, kvh = head / group, in_group = head % group;
+    const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int2 cut = items_cut[b * nkv + kvh];
+    const int units = cut.y;
+    if (units <= 1) return;
+    const int64_t rec = partial_floats(group, HD), step = nkv * rec;
+    const float* first = partial + cut.x * rec;
+    const float* m_of = first + group * HD + in_group;
+    if (threadIdx.x < 32) {
+        float top = -INFINITY;
+        for (int u = threadIdx.x; u < units; u += 32) top = fmaxf(top, m_of[u * step]);
+        top = warp_max(top);
+        if (threadIdx.x == 0) s_top = top;
+    }
+    __syncthreads();
+    const float top = s_top;
+    float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int u = slice; u < units; u += SLICES) {
+        const float4 v = *reinterpret_cast<const float4*>(first + u * step + in_group * HD + 4 * lane);
+        const float pl = m_of[u * step + group], f = part_weight(m_of[u * step], top, pl);
+        l += f * pl;
+        acc[0] += f * v.x; acc[1] += f * v.y; acc[2] += f * v.z; acc[3] += f * v.w;
+    }
+    *reinterpret_cast<float4*>(&s_o[slice][4 * lane]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (lane == 0) s_l[slice] = l;
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        float sum = 0.0f, o = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SLICES; i++) sum += s_l[i], o += s_o[i][threadIdx.x];
+        ((T*)a.out)[((int64_t)b * a.n_heads + head) * HD + threadIdx.x] = from_f32<T>(sum == 0.0f ? 0.0f : o / sum);
+    }
+}
+
 template <typename T, int HD, int NT>
 cudaError_t launch_nt(const Kv8DecodeArgs& a, cudaStream_t s) {
     int* counters = (int*)a.workspace;
     float* partial = (float*)((char*)a.workspace + kCounters * sizeof(int));
     const int64_t items = (int64_t)a.B * a.pool.n_kv_heads;
     const dim3 grid((unsigned)(items + units_wanted(items, kSms * kCtas<T, HD, NT>)));
-    return launch_ex(kv8_decode_kernel<T, HD, NT>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters);
+    const bool join = items <= kJoinItems && a.max_pages > kMinPages;
+    int2* items_cut = join ? (int2*)(partial + (items + kWaves * kSms * kMostCtas) * partial_floats(a.n_heads / a.pool.n_kv_heads, HD)) : nullptr;
+    const cudaError_t rc = launch_ex(kv8_decode_kernel<T, HD, NT>, grid, dim3(kWarps * 32), 0, s, 1, a, partial, counters, items_cut);
+    if (rc != cudaSuccess || !join) return rc;
+    count_launch();
+    return launch_ex(kv8_join_kernel<T, HD>, dim3((unsigned)a.B * a.n_heads), dim3(128), 0, s, 1, a, (const float*)partial, (const int2*)items_cut);
 }
 
 template <typename T, int HD>
@@ -571,7 +636,7 @@ size_t kv8_decode_workspace_bytes(int B, int n_heads, int n_kv_heads, int head_d
     const size_t rec = partial_floats(n_heads / n_kv_heads, head_dim) * sizeof(float);
     const int64_t items = (int64_t)B * n_kv_heads;
     const size_t n = items > kCounters ? 0 : (size_t)(items + kWaves * kSms * kMostCtas) * rec;
-    return kCounters * sizeof(int) + (n + 255) / 256 * 256;
+    return kCounters * sizeof(int) + (n + 255) / 256 * 256 + kJoinItems * sizeof(int2);
 }
 
 cudaError_t launch_kv8_decode(const Kv8DecodeArgs& a, cudaStream_t s) {
