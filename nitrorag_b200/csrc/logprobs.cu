@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 5) logprob_kern
 
     // the CTA's top k
     if (k) {
-        Key bound = full ? ~0ull : 0;  // fewer than 32 vectors: all their elements
+        Key bound = full ? ~0ull : 0;
         for (int w = 0; w < full; w++) bound = sh.warp_key[w] < bound ? sh.warp_key[w] : bound;
         const float least = bound ? key_value(bound) : -INFINITY;
         auto look = [&](const Vec& u, int v) {
@@ -394,7 +394,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 5) logprob_kern
             }
         };
         auto any = [&](int v) { return v >= w0 && v < w1 ? row.load_whole(v) : row.load(v); };
-        if (!bad && mine && mine >= bound) {
+        if (!full) {  // so few vectors that all their elements are ranked
+            const int64_t from = row.base(v0) < 0 ? 0 : row.base(v0);
+            const int n = (int)(min((int64_t)a.V, row.base(v1)) - from);
+            for (int i = t; i < n; i += kThreads) sh.keys[i] = rank_key(to_f32(row.p[from + i]), (int)(from + i));
+            if (t == 0) sh.count = max(n, 0);
+        } else if (!bad && mine && mine >= bound) {
             if (third >= least) {
                 sh.chosen[atomicAdd(&sh.n_chosen, 1)] = t;
             } else {
@@ -411,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 4 : 5) logprob_kern
                 for (int v = v0 + sh.chosen[c] + lane * kThreads; v < v1; v += 32 * kThreads) look(any(v), v);
             __syncthreads();
         }
-        if (bad || sh.count > kCandidates) {
+        if ((bad && full) || sh.count > kCandidates) {
             top_by_passes(row, v0, v1, k, sh);
         } else {
             // four threads to a candidate
