@@ -370,7 +370,8 @@ typedef struct nr_kv8_append_args {
  * rotation is two fp32 products and one fp32 sum per element, each rounded.  A block given a
  * non-finite value gets a NaN scale, so that attention over it gives NaN.  Codes behind a
  * sequence's last token are left as they were.
- * No two sequences of a call may append to the same page.  A sequence whose rows, positions
+ * A call may append to a page only once: not for two sequences, nor for two entries of one
+ * sequence's table.  max_pages <= 2^26.  A sequence whose rows, positions
  * (up to max_pages*16, and rope_len if rot_dim > 0) are out of range is skipped, and so is
  * the append of a page id outside [0, n_pages); both set *error_flag to 2.
  * q, k, v, q_out, k_out and strides must be 16-byte aligned; outputs may equal their input

@@ -697,7 +697,8 @@ static bool valid_rows(const void* p, int64_t stride, int64_t width, int32_t dty
 int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* g, int32_t* error_flag, void* stream) {
     nitro::Kv8AppendArgs a;
     if (!g || !read_kv8_pool(pool, g->layer, &a.pool) || !valid_dtype(g->dtype)) return NR_ERR_INVALID;
-    if (!g->cu_seqlens || !g->start_pos || !g->block_tables || g->B <= 0 || g->B > 1024 || g->T <= 0 || g->T > (1 << 30) || g->max_pages <= 0)
+    if (!g->cu_seqlens || !g->start_pos || !g->block_tables || g->B <= 0 || g->B > 1024 || g->T <= 0 || g->T > (1 << 30) || g->max_pages <= 0 ||
+        g->max_pages > (1 << 26))  // positions stay within 32 bits
         return NR_ERR_INVALID;
     const int hd = pool->head_dim;
     const int64_t kw = (int64_t)pool->n_kv_heads * hd, qw = (int64_t)g->n_heads * hd;

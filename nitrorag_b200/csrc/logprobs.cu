@@ -96,7 +96,7 @@ struct RowView {
     __device__ __forceinline__ Vec load_whole(int i) const { return load_whole_at(p + base(i)); }
     static __device__ __forceinline__ Vec load_whole_at(const T* at) {
         Vec v;
-        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                      : "=r"(v.u[0]), "=r"(v.u[1]), "=r"(v.u[2]), "=r"(v.u[3]), "=r"(v.u[4]), "=r"(v.u[5]), "=r"(v.u[6]), "=r"(v.u[7])
                      : "l"(at));
         return v;

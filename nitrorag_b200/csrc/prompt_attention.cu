@@ -250,7 +250,6 @@ __global__ void __launch_bounds__(Layout<HD, TILING>::kThreads, Layout<HD, TILIN
         tmem_relinquish();
     }
 
-
     // heads of one tile side by side (they share keys in L2), later tiles (more keys) of a
     // sequence first
     const int ny = TILING == kHeads ? a.n_heads / 2 : a.n_heads;

@@ -172,6 +172,16 @@ def test_graph_and_stream():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("H,KV", [(4, 2), (5, 5), (1, 1)])
+def test_long_among_short(dtype, H, KV):
+    """head_dim 128, 32 tokens and less on average, one of the sequences of many key blocks."""
+    lens = [1, 0, 3, 7, 2] * 20
+    lens[33] = 901
+    check(dtype, lens, lens, H, KV, 128, seed=H, pad=3)
+    check(dtype, [min(n, 140) for n in lens], lens, H, KV, 128, seed=H + 1)
+
+
 def test_many_sequences():
     rng = np.random.default_rng(1)
     check("bf16", rng.integers(0, 4, 1024).tolist(), rng.integers(0, 4, 1024).tolist(), 1, 1, 64, seed=5, pad=1)

@@ -40,6 +40,7 @@ def test_pools(kw):
     dict(rot_dim=-16), dict(rope_layout=2), dict(q=A + 2), dict(k=A + 8), dict(v=A + 4), dict(q_out=A + 2), dict(k_out=A + 2),
     dict(q_stride=255), dict(q_stride=248), dict(k_stride=127), dict(k_stride=132), dict(v_stride=0), dict(k_out_stride=64),
     dict(q_out_stride=264), dict(k_out_stride=136),  # in place with another stride
+    dict(max_pages=(1 << 26) + 1),  # 2^30 positions
 ])
 def test_append(kw):
     p, a = pool(), append_args(**kw)
@@ -58,7 +59,7 @@ DECODE = dict(q=A, dtype=1, layer=0, bt=A, max_pages=2, ctx=A, B=1, n_heads=4, o
 @pytest.mark.parametrize("kw", [
     dict(q=None), dict(bt=None), dict(ctx=None), dict(out=None), dict(ws=None), dict(dtype=3), dict(layer=2), dict(layer=-1),
     dict(max_pages=0), dict(B=0), dict(B=1025), dict(n_heads=0), dict(n_heads=3), dict(n_heads=34), dict(q=A + 2), dict(out=A + 8),
-    dict(ws=A + 4)])
+    dict(ws=A + 4), dict(max_pages=(1 << 26) + 1)])
 def test_decode(kw):
     p, d = pool(), {**DECODE, **kw}
     assert lib().nr_paged_attention_decode_kv8(d["q"], d["dtype"], C.byref(p), d["layer"], d["bt"], d["max_pages"], d["ctx"],
