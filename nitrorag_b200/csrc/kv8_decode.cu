@@ -31,7 +31,7 @@
 // items: 13.5 -> 10.2; but at 64 items 26.5 -> 27.0); else by the item's last CTA.
 //
 // Measured (of the copy bandwidth): 2 contexts of 131k tokens, 32 heads on 8, head_dim 128,
-// fp16: 104 us, 5.2 TB/s (0.79; the ALU, mostly the conversions of the codes, is at 46 %).  96
+// fp16: 104 us, 5.2 TB/s (0.79; issue slots are 40 % busy, mostly converting the codes).  96
 // contexts of 0..4096 tokens, the same heads: 100 us, 4.2 TB/s (0.64): a page's scales and
 // codes are addressed by a table entry that has to be read first, and a unit's start and end
 // read nothing.  64 contexts of 128..1024, 12 heads of 64, fp32: 25 us, 2.3 TB/s (0.35), of
