@@ -41,6 +41,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "kv8.h"
@@ -64,6 +65,7 @@ __host__ __device__ __forceinline__ int units_wanted(int64_t items, int slots) {
 // items to fill the device (64 sequences of 128..1024 tokens, 12 kv heads: 31 us with units
 // of 16 pages and up, 26.6 with 64).
 constexpr int kMinPages = 8, kMinPagesMany = 64;
+__host__ __device__ __forceinline__ int least_pages(int64_t items) { return items <= kSms ? kMinPages : kMinPagesMany; }
 // Items whose partial results can be counted; more items than that fill the device uncut.
 constexpr int kCounters = 16384;
 constexpr int kJoinItems = 32;  // most items whose parts a second kernel joins
@@ -332,7 +334,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kern
     const int wanted = units_wanted(items, kSms * kCtas<T, HD, NT>);
     const int64_t all = total * nkv;
     const int per = all <= INT32_MAX - wanted ? ((int)all + wanted - 1) / wanted : (int)min((all + wanted - 1) / wanted, (int64_t)INT32_MAX);
-    const int chunk = items > kCounters ? INT32_MAX : max(items <= kSms ? kMinPages : kMinPagesMany, per);
+    const int chunk = items > kCounters ? INT32_MAX : max(least_pages(items), per);
     const int unit = blockIdx.x;
     int b = -1, pages = 0, units = 0, at = 0;  // at: first unit of sequence b
     for (int i0 = 0, before = 0; i0 < a.B && b < 0; i0 += 32) {
@@ -611,7 +613,10 @@ cudaError_t launch_nt(const Kv8DecodeArgs& a, cudaStream_t s) {
     int* counters = (int*)a.workspace;
     float* partial = (float*)((char*)a.workspace + kCounters * sizeof(int));
     const int64_t items = (int64_t)a.B * a.pool.n_kv_heads;
-    const dim3 grid((unsigned)(items + units_wanted(items, kSms * kCtas<T, HD, NT>)));
+    // No more CTAs than the table has room for units: an idle one takes the time of its look at
+    // the lengths.
+    const int64_t most = items > kCounters ? items : items * ((a.max_pages - 1) / least_pages(items) + 1);
+    const dim3 grid((unsigned)std::min(items + units_wanted(items, kSms * kCtas<T, HD, NT>), most));
     // Up to 8 parts are loaded at once by the last CTA: not worth a second launch (601 tokens, 12
     // items: 8.7 us a call, 10.1 with it).
     const bool join = items <= kJoinItems && a.max_pages > 8 * kMinPages;
