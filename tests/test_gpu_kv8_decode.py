@@ -192,3 +192,24 @@ def test_workspace_is_left_ready_and_can_be_shared_in_order():
         graph.replay()
         assert torch.equal(out, want[0])
         assert torch.equal(decode(a[0], a[3], a[1], a[2], ws=ws), want[0])
+
+
+@pytest.mark.parametrize("H,KV,hd", [(2, 2, 64), (16, 1, 128), (14, 2, 64)])
+def test_long_contexts_of_few_sequences(H, KV, hd):
+    """Items of many parts, one of few and an empty one in a wide table: a page outside the pool, then a
+    NaN block, which reach their own sequence and heads only."""
+    rng = np.random.default_rng(H)
+    ctx = [5003, 0, 37, 4096, 1]
+    counts = [(n + PAGE - 1) // PAGE for n in ctx]
+    pool = Pool(sum(counts), 1, KV, hd, seed=H)
+    table = tables(rng, counts, sum(counts))
+    q = torch.randn((5, H, hd), device="cuda")
+    sound = check(pool, q, table, i32(ctx), 0, "f32")
+    bad = table.clone()
+    bad[3, 100] = -1
+    got = check(pool, q, bad, i32(ctx), 0, "f32", flag=2)
+    assert torch.equal(got[:3], sound[:3]) and torch.equal(got[4], sound[4])
+    pool.v_scale[int(table[0, 200]), 0, KV - 1] = float("nan")
+    got = decode(pool, q, table, i32(ctx))
+    assert bool(got[0, -(H // KV):].isnan().all()) and torch.equal(got[1:], sound[1:])
+    assert torch.equal(got[0, :-(H // KV)], sound[0, :-(H // KV)])
