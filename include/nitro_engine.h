@@ -384,7 +384,8 @@ int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* args, int32
  * out of range is clamped, a page id outside [0, n_pages) counts as 16 absent tokens; both
  * set *error_flag to 2.  n_heads <= 16 * n_kv_heads.  q, out and workspace 16-byte aligned.
  * workspace: nr_paged_attention_kv8_workspace_size() bytes, zero before the first call (each
- * call leaves its counters zero again); calls that may overlap on the device need one each. */
+ * call leaves its counters zero again); calls that may overlap on the device need one each.
+ * The size does not fall as B grows, so one for the largest batch serves all smaller ones. */
 size_t nr_paged_attention_kv8_workspace_size(int32_t B, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
                                              int32_t max_pages);
 int nr_paged_attention_decode_kv8(const void* q, int32_t dtype, const nr_kv8_pool* pool, int32_t layer,

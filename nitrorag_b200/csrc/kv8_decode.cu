@@ -641,8 +641,10 @@ cudaError_t launch_t(const Kv8DecodeArgs& a, cudaStream_t s) {
 
 size_t kv8_decode_workspace_bytes(int B, int n_heads, int n_kv_heads, int head_dim, int) {
     const size_t rec = partial_floats(n_heads / n_kv_heads, head_dim) * sizeof(float);
-    const int64_t items = (int64_t)B * n_kv_heads;
-    const size_t n = items > kCounters ? 0 : (size_t)(items + kWaves * kSms * kMostCtas) * rec;
+    // the largest cut batch up to B: what holds a batch holds every smaller one, also where B's own
+    // items are past the counters and need no partial results
+    const int64_t items = std::min(B, kCounters / n_kv_heads) * (int64_t)n_kv_heads;
+    const size_t n = items ? (size_t)(items + kWaves * kSms * kMostCtas) * rec : 0;
     return kCounters * sizeof(int) + (n + 255) / 256 * 256 + kJoinItems * sizeof(int2);
 }
 

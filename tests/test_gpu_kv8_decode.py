@@ -213,3 +213,42 @@ def test_long_contexts_of_few_sequences(H, KV, hd):
     got = decode(pool, q, table, i32(ctx))
     assert bool(got[0, -(H // KV):].isnan().all()) and torch.equal(got[1:], sound[1:])
     assert torch.equal(got[0, :-(H // KV)], sound[0, :-(H // KV)])
+
+
+def few_pages(B, KV, hd, ctx, width, seed, P=200):
+    """A pool that many short contexts share, and tables into it of any pages."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    pool = Pool(P, 1, KV, hd, seed=seed)
+    return pool, torch.randint(0, P, (B, width), generator=g, device="cuda", dtype=torch.int32), i32(ctx)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,H,KV,hd,most", [(19, 16, 8, 128, 2100), (75, 4, 2, 64, 1500), (300, 3, 3, 64, 700)])
+def test_many_items(dtype, B, H, KV, hd, most):
+    """Over 148 (sequence, kv head) items, where a unit has 64 pages at least: contexts of several units,
+    of one and of none side by side; those that pass a narrow table are clamped and flagged."""
+    rng = np.random.default_rng(B)
+    ctx = [most - 3, 0, 1, 1024, 1025] + rng.integers(0, most, B - 5).tolist()
+    pool, table, lens = few_pages(B, KV, hd, ctx, (most + PAGE - 1) // PAGE, seed=B)
+    q = torch.randn((B, H, hd), device="cuda").to(DTYPES[dtype][1])
+    check(pool, q, table, lens, 0, dtype, flag=2 if max(ctx) > table.shape[1] * PAGE else 0)
+
+
+def test_one_workspace_of_the_largest_batch():
+    """A workspace sized for 1024 sequences of 17 kv heads, whose items are past the counters and stay
+    uncut, serves smaller batches that are cut; what lies behind it is not touched."""
+    H, KV, hd, width = 17, 17, 64, 130
+    size = lib().nr_paged_attention_kv8_workspace_size(1024, H, KV, hd, width)
+    ws = torch.zeros(size + 4096, dtype=torch.uint8, device="cuda")
+    ws[size:] = 0xa5
+    rng = np.random.default_rng(4)
+    for B in (1024, 960, 30, 1):
+        ctx = rng.integers(0, 60, B)
+        ctx[0] = width * PAGE - 5
+        pool, table, lens = few_pages(B, KV, hd, ctx.tolist(), width, seed=B, P=400)
+        q = torch.randn((B, H, hd), device="cuda")
+        got = decode(pool, q, table, lens, ws=ws)
+        some = list(range(min(B, 40)))
+        want, pv, size_ = reference(pool, q[some], table[some], lens[some], 0)
+        assert_within(got[some], want, bound("f32", want, pv, size_, P_ROUND["f32"]), "decode")
+        assert bool((ws[size:] == 0xa5).all())

@@ -75,6 +75,21 @@ def test_decode_workspace_size():
         assert size(*bad) == 0
 
 
+@pytest.mark.parametrize("H,KV,hd", [(32, 32, 128), (17, 17, 64), (32, 8, 128), (16, 1, 64), (20000, 20000, 64)])
+def test_decode_workspace_size_never_falls_with_the_batch(H, KV, hd):
+    """One workspace, sized for the largest batch, serves every smaller one: the sizes never fall, and each
+    holds the counters, a partial result for each unit of a batch that is cut (up to 16384 items of a
+    sequence and kv head are), and the list of units of up to 32 items."""
+    group, before = H // KV, 0
+    rec = (group * hd + (2 * group + 3) // 4 * 4) * 4
+    for b in range(1, 1025):
+        size = lib().nr_paged_attention_kv8_workspace_size(b, H, KV, hd, 2048)
+        assert size >= before
+        before = size
+        items = b * KV
+        assert size >= 4 * 16384 + ((items + 2 * 148 * 5) * rec if items <= 16384 else 0) + (8 * items if items <= 32 else 0)
+
+
 PROMPT = dict(q=A, qs=256, k=A, ks=128, v=A, vs=128, out=A, os=256, dtype=1, cu_q=A, cu_k=None, B=1, Tq=8, Tk=8, H=4, KV=2, hd=64)
 
 
