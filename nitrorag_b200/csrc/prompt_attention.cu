@@ -446,6 +446,9 @@ __global__ void __launch_bounds__(Layout<HD, TILING>::kThreads, Layout<HD, TILIN
                         tmem_st16(to + c, w);
                     }
                 }
+                // stores to the same columns are not ordered among themselves: the old maximum's
+                // weights have to be there before the new one's go over them
+                tmem_wait_st();
                 moved = true;
             }
             tmem_wait_st();

@@ -185,3 +185,28 @@ def test_long_among_short(dtype, H, KV):
 def test_many_sequences():
     rng = np.random.default_rng(1)
     check("bf16", rng.integers(0, 4, 1024).tolist(), rng.integers(0, 4, 1024).tolist(), 1, 1, 64, seed=5, pad=1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("lens,H,KV,hd", [([700, 130], 4, 2, 128), ([700, 130], 3, 3, 128), ([5] * 60 + [290], 2, 1, 128),
+                                          ([700, 130], 4, 2, 64)])
+@pytest.mark.parametrize("level,step", [(-60, 0), (60, 0), (-90, 12), (90, -12), (0, 12)])
+def test_weights_of_the_old_maximum_never_stay(dtype, lens, H, KV, hd, level, step):
+    """Scores near `level` that move by `step` from one block of 128 keys to the next: the weights taken
+    from the maximum so far (0 before the first block) would be infinite or nothing, so that one of
+    them left among the new maximum's shows.  Every tiling: two heads, two tiles of a head, one tile."""
+    dt = DTYPES[dtype][1]
+    g = torch.Generator(device="cuda").manual_seed(hd + H + len(lens))
+    n = sum(lens)
+    q = (0.05 * torch.randn((n, H, hd), generator=g, device="cuda"))
+    k = torch.randn((n, KV, hd), generator=g, device="cuda")
+    at = torch.cat([torch.arange(m, device="cuda") for m in lens])
+    q[:, :, 0] = 8.0  # the score's level, in one dim: 8 k / sqrt(hd)
+    k[:, :, 0] = ((level + step * (at // 128)).float() * hd ** 0.5 / 8.0)[:, None]
+    q, k = q.to(dt).reshape(n, -1), k.to(dt).reshape(n, -1)
+    v = torch.randn((n, KV * hd), generator=g, device="cuda").to(dt)
+    cu = i32([0] + np.cumsum(lens).tolist())
+    out = torch.full_like(q, 5.0)
+    call(q, k, v, out, cu, None, len(lens), H, KV, hd)
+    want, scores, small = reference(q, k, v, lens, lens, H, KV, hd)
+    assert_within(out.reshape(n, H, hd), want, bound(dtype, want, *scores, P_ROUND[dtype], small), "prompt")
