@@ -252,3 +252,29 @@ def test_one_workspace_of_the_largest_batch():
         want, pv, size_ = reference(pool, q[some], table[some], lens[some], 0)
         assert_within(got[some], want, bound("f32", want, pv, size_, P_ROUND["f32"]), "decode")
         assert bool((ws[size:] == 0xa5).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("B", [1, 5])  # parts joined by the second kernel, by an item's last CTA
+@pytest.mark.parametrize("what", ["k_scale", "v_scale"])
+def test_nan_block_of_no_weight(dtype, B, what):
+    """A block with a NaN scale among tokens whose weights are 0 in fp32: its sequence and head are NaN
+    however the context is cut, the others as without it."""
+    hd, H, KV = 64, 16, 8
+    ctx = [2000, 5, 1, 0, 33][:B]
+    counts = [(n + PAGE - 1) // PAGE for n in ctx]
+    pool = Pool(sum(counts), 1, KV, hd, seed=B)
+    table = tables(np.random.default_rng(B), counts, sum(counts))
+    q = torch.randn((B, H, hd), device="cuda", generator=torch.Generator(device="cuda").manual_seed(B))
+    q[:, :, 0] = 8.0
+    first = table[0, :8].long()  # scores of -112: weights of e^-112 and less
+    pool.k[first] = 0
+    pool.k[first, :, :, :, 0] = 0xfe  # -448
+    pool.k_scale[first] = 0.25
+    q = q.to(DTYPES[dtype][1])
+    sound = check(pool, q, table, i32(ctx), 0, dtype)
+    getattr(pool, what)[first[2], 0, 3] = float("nan")
+    got = decode(pool, q, table, i32(ctx))
+    assert bool(got[0, 6:8].isnan().all())
+    got[0, 6:8] = sound[0, 6:8]
+    assert torch.equal(got, sound)
