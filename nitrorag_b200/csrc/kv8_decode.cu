@@ -553,9 +553,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<T, HD, NT>) kv8_decode_kern
             }
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-                if (u0 + i >= units) break;
-                const float f = part_weight(m[i], top, l[i]);  // 0 too: a NaN reaches the row whatever its weight
-                acc[0] += f * v[i].x; acc[1] += f * v[i].y; acc[2] += f * v[i].z; acc[3] += f * v[i].w;
+                // a weight of 0 too: a NaN reaches the row whatever its weight
+                const float f = u0 + i < units ? part_weight(m[i], top, l[i]) : 0.0f;
+                if (u0 + i < units) {
+                    acc[0] += f * v[i].x; acc[1] += f * v[i].y; acc[2] += f * v[i].z; acc[3] += f * v[i].w;
+                }
             }
         }
 #pragma unroll
