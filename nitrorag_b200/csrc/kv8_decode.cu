@@ -245,7 +245,7 @@ struct WarpState {
             for (int i = 0; i < 4; i++) {
                 const float p = exp2_fast(s[n][i] - m[n][i & 1]);
                 l[n][i & 1] += p;
-                w[i] = p * (vs * gain[n][i & 1]);
+                w[i] = p * vs * gain[n][i & 1];  // vs * gain alone may pass the range: a scale of 2^-126 so far
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {

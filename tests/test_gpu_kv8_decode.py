@@ -278,3 +278,29 @@ def test_nan_block_of_no_weight(dtype, B, what):
     assert bool(got[0, 6:8].isnan().all())
     got[0, 6:8] = sound[0, 6:8]
     assert torch.equal(got, sound)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,H,KV", [(64, 4, 2), (128, 12, 1)])
+@pytest.mark.parametrize("large", [16.0, 2.0 ** 60])
+def test_values_of_nothing_before_large_ones(dtype, hd, H, KV, large):
+    """Blocks of zero values (scale 2^-126) with all the weight, then large values whose weights are 0 in
+    fp32: no product of the two scales leaves the range."""
+    pool = Pool(12, 1, KV, hd, seed=hd)
+    table = i32([list(range(12))])
+    q = torch.randn((1, H, hd), device="cuda", generator=torch.Generator(device="cuda").manual_seed(hd))
+    q[:, :, 0] = 8.0
+    q = q.to(DTYPES[dtype][1])
+    pool.v[:8] = 0
+    pool.v_scale[:8] = 2.0 ** -126
+    pool.k[8:] = 0
+    pool.k[8:, :, :, :, 0] = 0xfe  # -448: scores of -112 or -79, where the others are near 0
+    pool.k_scale[8:] = 0.25
+    pool.v_scale[8:] = large
+    for first in (pool.v[:8], Pool(8, 1, KV, hd, seed=1).v):  # none, then values of 2^-117 and less
+        pool.v[:8] = first
+        got, (want, pv, size) = decode(pool, q, table, i32([12 * PAGE - 3])), reference(pool, q, table, [12 * PAGE - 3], 0)
+        # weights are fp32 without its subnormals: what e^(s - m) < 2^-126 multiplies is lost, at most
+        # 2^-126 sum |v|
+        lost = 2.0 ** -126 * pool.values("v").abs().sum((0, 1, 3)).repeat_interleave(H // KV, 0)[None]
+        assert_within(got, want, bound(dtype, want, pv, size, P_ROUND[dtype]) + lost, "decode")
