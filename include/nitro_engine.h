@@ -311,7 +311,13 @@ int nr_q8_matmul(const float* x, const int8_t* q, const float* scales, float* ou
  * above, asynchronous, no allocation and no host synchronisation, so every call can be
  * captured into a CUDA graph (make the first call on each device outside a capture).  Each
  * call runs on the current device, which must be the stream's.  Sums, softmax statistics
- * and rotations are fp32; 16-bit outputs are rounded once.
+ * and rotations are fp32; 16-bit outputs are rounded once.  Beside that the attention
+ * calls round the operands of their products: nr_prompt_attention a weight to the inputs' type;
+ * the decode over 8-bit pages query and weights to fp16, scaled by powers of two (relative
+ * 2^-11; 2^-22 from two halves with fp32 inputs; never more than 2^-32 of the row's largest).
+ * Their sums of weights (up to 2^8 each) times values are divided by the weights' sum at the
+ * end: |value| times the context length has to stay below 2^119.
+ * B <= 1024 throughout.
  *
  * Element type of the q, k, v, logits and attention outputs of these entry points. */
 #define NR_DTYPE_F32   0

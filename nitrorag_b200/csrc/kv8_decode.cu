@@ -14,12 +14,15 @@
 //
 // fp16 has few exponent bits, so both small operands are scaled by powers of two (exact):
 // a query row to a largest value of 2^7, and the weights W = p * v_scale * gain with a gain
-// per head that puts the largest weight so far near 2^7, so that what matters in the sum
-// is never below fp16's normal range whatever the blocks' scales are.  p = exp2(s - m) goes by a
+// per head that puts the largest weight so far near 2^7, whatever the blocks' scales are.
+// Weights down to 2^-21 of the largest keep fp16's relative precision, smaller ones are off by
+// at most 2^-32 of the largest (which shows only in a dim where the tokens with the large
+// weights have no values).  p = exp2(s - m) goes by a
 // running maximum that is only moved when a score passes it by 8 (a weight of at most 2^8
 // costs no precision), so most pages need no exchange between lanes.  16-bit inputs round
-// a weight once to fp16 (2^-11, under the output's own rounding); fp32 inputs carry query
-// and weights as two fp16 halves (22 bits) and take each product twice.
+// a weight once to fp16 (2^-11, under a bf16 output's own rounding and as much as an fp16
+// one's); fp32 inputs carry query and weights as two fp16 halves (22 bits) and take each
+// product twice.
 //
 // Work: the pages of all (sequence, kv head) items are cut into units of about equal
 // length, one CTA each, its four warps taking every fourth page.  The cut goes by the

@@ -304,3 +304,43 @@ def test_values_of_nothing_before_large_ones(dtype, hd, H, KV, large):
         # 2^-126 sum |v|
         lost = 2.0 ** -126 * pool.values("v").abs().sum((0, 1, 3)).repeat_interleave(H // KV, 0)[None]
         assert_within(got, want, bound(dtype, want, pv, size, P_ROUND[dtype]) + lost, "decode")
+
+
+def lost_weights(pool, q, table, ctx, layer):
+    """What the weights' 16-bit form may lose: they enter the product in units in which the largest of
+    p v_scale so far is at least 2^7, and an fp16 number is off by 2^-25 at most below its normal
+    range: 2^-32 of the largest, of each |code|.  The second half of an fp32 weight is no finer there."""
+    B, H, hd = q.shape
+    KV = pool.shape4[2]
+    out = torch.zeros((B, H, hd), dtype=torch.float64, device="cuda")
+    for b in range(B):
+        n = int(ctx[b])
+        ids = table[b, :(n + PAGE - 1) // PAGE].long()
+        for j in range(KV):
+            kk = pool.values("k")[ids, layer, j].reshape(-1, hd)[:n]
+            codes = pool.v[ids, layer, j].view(torch.float8_e4m3fn).double().reshape(-1, hd)[:n].abs().sum(0)
+            vs = pool.v_scale[ids, layer, j].double().repeat_interleave(PAGE)[:n]
+            g = H // KV
+            p = torch.softmax(q[b, j * g:(j + 1) * g].double() @ kk.T / hd ** 0.5, -1)
+            if n:
+                out[b, j * g:(j + 1) * g] = 2.0 ** -32 * (p * vs).amax(-1, keepdim=True) * codes
+    return out
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd,H,KV", [(64, 4, 2), (128, 9, 1)])
+def test_weights_far_below_the_largest(dtype, hd, H, KV):
+    """Few tokens have nearly all the weight, and no values in half of the dims, where only tokens of
+    weights down to 2^-60 of theirs count."""
+    ctx = [7, 100, 333]
+    pool = Pool(63, 1, KV, hd, seed=hd)
+    g = torch.Generator(device="cuda").manual_seed(H)
+    table = torch.arange(63, device="cuda", dtype=torch.int32).reshape(3, 21)
+    q = torch.randn((3, H, hd), device="cuda", generator=g)
+    q[:, :, 0] = 8.0
+    q = q.to(DTYPES[dtype][1])
+    pool.k[:, :, :, :, 0] = torch.randint(0x10, 0x7e, (63, 1, KV, PAGE), device="cuda", generator=g).to(torch.uint8) + 128
+    pool.k[:, :, :, 3, 0] = 0
+    pool.v[:, :, :, 3, :hd // 2] = 0
+    got, (want, pv, size) = decode(pool, q, table, i32(ctx)), reference(pool, q, table, ctx, 0)
+    assert_within(got, want, bound(dtype, want, pv, size, P_ROUND[dtype]) + lost_weights(pool, q, table, ctx, 0), "decode")
