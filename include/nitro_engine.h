@@ -313,8 +313,9 @@ int nr_q8_matmul(const float* x, const int8_t* q, const float* scales, float* ou
  * call runs on the current device, which must be the stream's.  Sums, softmax statistics
  * and rotations are fp32; 16-bit outputs are rounded once.  Beside that the attention
  * calls round the operands of their products: nr_prompt_attention a weight to the inputs' type;
- * the decode over 8-bit pages query and weights to fp16, scaled by powers of two (relative
- * 2^-11; 2^-22 from two halves with fp32 inputs; never more than 2^-32 of the row's largest).
+ * the decode over 8-bit pages query and weights to fp16, scaled by powers of two (off by 2^-11
+ * of the value, 2^-22 with fp32 inputs, which are taken as two halves, or by 2^-32 of the row's
+ * largest where that is more).
  * Their sums of weights (up to 2^8 each) times values are divided by the weights' sum at the
  * end: |value| times the context length has to stay below 2^119.
  * B <= 1024 throughout.
@@ -379,7 +380,8 @@ typedef struct nr_kv8_append_args {
  * A call may append to a page only once: not for two sequences, nor for two entries of one
  * sequence's table.  max_pages <= 2^26.  A sequence whose rows, positions
  * (up to max_pages*16, and rope_len if rot_dim > 0) are out of range is skipped, and so is
- * the append of a page id outside [0, n_pages); both set *error_flag to 2.
+ * the append of a page id outside [0, n_pages); both set *error_flag to 2.  Where cu_seqlens
+ * decreases the flag is set too, but sequences beside that place may be skipped with it.
  * q, k, v, q_out, k_out and strides must be 16-byte aligned; outputs may equal their input
  * (same stride) and overlap nothing else. */
 int nr_kv8_append(const nr_kv8_pool* pool, const nr_kv8_append_args* args, int32_t* error_flag, void* stream);
@@ -400,7 +402,9 @@ int nr_paged_attention_decode_kv8(const void* q, int32_t dtype, const nr_kv8_poo
                                   void* stream);
 
 /* Causal attention over whole prompts: B sequences packed in rows, q rows cu_q[b] ..
- * cu_q[b+1]-1 against k, v rows cu_k[b] .. cu_k[b+1]-1 (cu_k NULL: cu_q).  The last query of
+ * cu_q[b+1]-1 against k, v rows cu_k[b] .. cu_k[b+1]-1 (cu_k NULL: cu_q).  cu_q does not
+ * decrease (where it does, *error_flag is set to 2, and sequences beside that place may be
+ * skipped too).  The last query of
  * a sequence sees all its keys, each earlier one a key less; a query that sees none gives a
  * zero row.  q, out rows hold n_heads*head_dim elements, k, v rows n_kv_heads*head_dim, at
  * the given row strides (in elements); scores are scaled by 1/sqrt(head_dim).  dtype

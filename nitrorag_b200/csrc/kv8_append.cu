@@ -16,10 +16,10 @@
 // The maximum is taken over the bits of |x| as unsigned numbers, in which infinities and
 // NaNs are largest: they reach the scale, which becomes NaN.
 //
-// Measured: 12 prompts of 33..1300 tokens (8k together), 32 heads on 8 of 128, bf16: 48 us,
-// 5.1 TB/s, 0.78 of the measured copy bandwidth; reads and writes alternate in each warp,
+// Measured: 12 prompts of 33..1300 tokens (8k together), 32 heads on 8 of 128, bf16: 49 us,
+// 5.0 TB/s, 0.76 of the measured copy bandwidth; reads and writes alternate in each warp,
 // and issue slots are a third to half busy with the rotation and the conversions.  One token
-// of 64 sequences: 7.0 us, of one: 3.3 us, the chain from the lengths over the page table to
+// of 61 sequences: 7.4 us, of one: 3.6 us, the chain from the lengths over the page table to
 // the page (a call costs the host 8 us).  A CTA for each unit and head, the tile in fp32: 80 us
 // (a lane's 64 values leave registers for few warps).
 #include <cuda_fp8.h>

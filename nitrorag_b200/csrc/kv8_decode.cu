@@ -35,10 +35,11 @@
 //
 // Measured (of the copy bandwidth): 2 contexts of 131k tokens, 32 heads on 8, head_dim 128,
 // fp16: 104 us, 5.2 TB/s (0.79; issue slots are 40 % busy, mostly converting the codes).  96
-// contexts of 0..4096 tokens, the same heads: 100 us, 4.2 TB/s (0.64): a page's scales and
+// contexts of 0..4096 tokens, the same heads: 101 us, 4.2 TB/s (0.64): a page's scales and
 // codes are addressed by a table entry that has to be read first, and a unit's start and end
-// read nothing.  64 contexts of 128..1024, 12 heads of 64, fp32: 25 us, 2.3 TB/s (0.35), of
-// which about 8 us are a single unit's chain of latencies, as one context of 601 tokens takes.
+// read nothing.  64 contexts of 128..1024, 12 heads of 64, fp32: 25 us, 2.3 TB/s (0.35): each
+// item is one unit, and a warp of the longest takes its 16 pages one after another.  One
+// context of 601 tokens: 8 us, a unit's chain of latencies.
 // Tried and left: runs of equal length over item borders, several items' pieces to a CTA
 // (27 -> 36, 100 -> 115 us: the pieces' latencies come one after another).
 #include <cuda_fp8.h>
@@ -64,9 +65,13 @@ constexpr int kSms = 148, kMostCtas = 5;
 __host__ __device__ __forceinline__ int units_wanted(int64_t items, int slots) {
     return items <= slots / 2 ? slots - (int)items : kWaves * slots;
 }
-// A unit's least pages: two for each warp where units are few, more where there are enough
-// items to fill the device (64 sequences of 128..1024 tokens, 12 kv heads: 31 us with units
-// of 16 pages and up, 26.6 with 64).
+// A unit's least pages: two for each warp where items are few, more where items alone fill the
+// device.  With 8 and with 64 pages at least, 8 kv heads of 128, bf16, 1000 tokens: 16 / 18
+// sequences 14.5 / 16.4 us with 8 (what the rule takes); 19 / 24 / 32: 16.5 / 17.1 / 20.6
+// with 8, 23.5 / 24.5 / 26.3 with 64 (taken); 48 / 64: 32.7 / 43.6 with 8, 30.1 / 30.9 with 64
+// (taken).  12 heads of 64, fp32, 128..1024 tokens: 24 sequences 14.6 and 20.6 (taken), 32:
+// 23.7 and 22.1 (taken), 64: 31.3 and 24.7 (taken).  So from 149 to about 300 items, half the
+// CTAs that run at once, the rule takes the slower side.
 constexpr int kMinPages = 8, kMinPagesMany = 64;
 __host__ __device__ __forceinline__ int least_pages(int64_t items) { return items <= kSms ? kMinPages : kMinPagesMany; }
 // Items whose partial results can be counted; more items than that fill the device uncut.

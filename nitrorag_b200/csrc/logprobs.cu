@@ -20,7 +20,7 @@
 // NaN and more candidates than the buffer holds take k passes instead.
 //
 // Measured: 2048 rows of 128256 bf16 logits, top 20: 111 us, 4.74 TB/s, 0.72 of the measured copy
-// bandwidth (98 us without a top list; fp32 logits 6.0 TB/s, 0.92): two elements of 16 bits
+// bandwidth (98 us without a top list; 1024 rows of fp32 logits 5.5 TB/s, 0.84, without a list 6.0, 0.92): two elements of 16 bits
 // for each of 32 need twice the exponentials (8 cycles a warp) and sums for the same bytes,
 // and the candidates' latency is hidden only by the SM's other rows.  64 rows of 32000 fp32:
 // 9.2 us, a chain of latencies.  A ninth warp that finishes a row while the others stream

@@ -34,7 +34,7 @@
 // saved no time).  Per 128-key step of both tiles the tensor cores need 2300 cycles (the first
 // product 640, bound by reading both operands from shared memory, the second 512, twice), the
 // special function unit 2100, a step takes 3000.  head_dim 64 has half the products for the
-// same exponentials: 557 TFLOP/s at 8192 tokens.  Tried and left: a product warp for each
+// same exponentials: 664 TFLOP/s at 8192 tokens, 32 heads on 8.  Tried and left: a product warp for each
 // tile (their products interleave: 485 us), two threads to a row (497), exponentials partly by
 // polynomial (437: the issue slots it takes are the ones that are short), S read twice
 // instead of a row in registers (473).
@@ -560,7 +560,9 @@ cudaError_t launch_t(const PromptAttnArgs& a, cudaStream_t s) {
     if (a.head_dim == 64) return launch_tiles<T, 64, kOne>(a, s);
     // Prompts of 32 keys and less on average: a CTA lives a few microseconds and waits most of
     // them, so two smaller ones to an SM, each with one block of rows (32 prompts of 7 tokens, 21
-    // heads: 27.8 -> 17.3 us; 64 of 40, 32 heads: 58.5 -> 56.5; but 8 of 64: 9.5 -> 11.9).
+    // heads: 27.8 -> 17.3 us; 64 of 40, 32 heads: 58.5 -> 56.5; but 8 of 64: 9.5 -> 11.9).  The
+    // average is what the host knows: a long prompt among many of one token pays for it (63 of
+    // one and one of 1900, 32 heads: 81 us, the long one alone 35).
     if (a.Tk / a.B <= 32) return launch_tiles<T, 128, kOne>(a, s);
     return a.n_heads / a.n_kv_heads % 2 ? launch_tiles<T, 128, kRows>(a, s) : launch_tiles<T, 128, kHeads>(a, s);
 }
