@@ -261,3 +261,39 @@ def test_graph_replay_and_other_stream():
     torch.cuda.synchronize()
     same_pool(pool, want)
     assert torch.equal(q_out, second)
+
+
+def test_offsets_past_32_bits():
+    """Pages at the far end of a pool of more than 2^32 codes, and rows past element 2^31 of their tensor."""
+    H, KV, hd, layers, rot = 2, 8, 128, 4, 64
+    P = (1 << 32) // (layers * KV * PAGE * hd) + 20
+    pool = Pool.__new__(Pool)
+    pool.shape4 = (P, layers, KV, hd)
+    for n in "kv":
+        setattr(pool, n, torch.zeros((P, layers, KV, PAGE, hd), dtype=torch.uint8, device="cuda"))
+        setattr(pool, n + "_scale", torch.ones((P, layers, KV), device="cuda"))
+    small = Pool(20, layers, KV, hd, zero=True)
+    for n in "kv":
+        getattr(small, n + "_scale").fill_(1.0)
+    width = (H + 2 * KV) * hd
+    rows = torch.zeros(((1 << 31) // width + 100, width), dtype=torch.bfloat16, device="cuda")
+    lens, start = [37, 21], [5, 16]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows[-sum(lens):] = torch.randn((sum(lens), width), generator=g, device="cuda").to(rows.dtype)
+    cos, sin = rope(64, rot)
+    cu = i32([0] + np.cumsum(lens).tolist())
+    near = torch.arange(20, device="cuda", dtype=torch.int32).reshape(2, 10)
+    kw = dict(rot=rot, layout=1, cos=cos, sin=sin, layer=3, n_heads=H)
+
+    def go(p, rows, cu, table):
+        q, k, v = rows[:, :H * hd], rows[:, H * hd:(H + KV) * hd], rows[:, (H + KV) * hd:]
+        err = i32([0])
+        append(p, q, k, v, cu, i32(start), table, q_out=q, k_out=k, err=err, **kw)  # in place
+        assert int(err) == 0
+
+    last = rows[-sum(lens):].clone()
+    go(small, last, cu, near)
+    go(pool, rows, cu + (len(rows) - sum(lens)), near + (P - 20))
+    assert torch.equal(rows[-sum(lens):], last)
+    for n in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(pool, n)[-20:], getattr(small, n)), n

@@ -344,3 +344,31 @@ def test_weights_far_below_the_largest(dtype, hd, H, KV):
     pool.v[:, :, :, 3, :hd // 2] = 0
     got, (want, pv, size) = decode(pool, q, table, i32(ctx)), reference(pool, q, table, ctx, 0)
     assert_within(got, want, bound(dtype, want, pv, size, P_ROUND[dtype]) + lost_weights(pool, q, table, ctx, 0), "decode")
+
+
+@pytest.mark.parametrize("B,H,KV,width", [(2, 16, 2, 200), (6, 8, 8, 200), (40, 8, 8, 80)])
+def test_graph_replay_with_other_lengths(B, H, KV, width):
+    """A captured call replayed with contexts and tables that were not there at the capture, on the
+    paths of both joins and of whole items; two such graphs share a workspace, one after the other."""
+    hd = 64
+    rng = np.random.default_rng(B)
+    pool, table, lens = few_pages(B, KV, hd, [1] * B, width, seed=B)
+    q = torch.randn((B, H, hd), device="cuda")
+    size = lib().nr_paged_attention_kv8_workspace_size(B, H, KV, hd, width)
+    ws, outs = torch.zeros(size, dtype=torch.uint8, device="cuda"), [torch.zeros_like(q) for _ in range(2)]
+    decode(pool, q, table, lens, out=outs[0], ws=ws)
+    torch.cuda.synchronize()
+    graphs = []
+    for out in outs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            decode(pool, q, table, lens, out=out, ws=ws)
+    for longest in (width * PAGE, 5, 0, width * PAGE - 7):
+        lens.copy_(i32(rng.integers(0, longest + 1, B).tolist()))
+        lens[-1] = longest
+        table.copy_(table.flip(0).clone())
+        for graph in graphs:
+            graph.replay()
+        want, pv, size_ = reference(pool, q, table, lens, 0)
+        assert_within(outs[0], want, bound("f32", want, pv, size_, P_ROUND["f32"]), "replayed")
+        assert torch.equal(outs[0], outs[1])

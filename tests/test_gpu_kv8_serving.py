@@ -148,3 +148,41 @@ def test_engine_last_decode_logprobs(tiny_model):
     with pytest.raises(NrError):
         eng.last_decode_logprobs(top_k=1)
     eng.close()
+
+
+def test_two_streams_at_once():
+    """Prompts of both head sizes, decode and log probabilities on two streams side by side, each stream
+    with its own workspace and outputs: what each gives alone."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rand = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    work = []
+    for hd, H, KV, lens in ((64, 12, 12, [300, 41, 700]), (128, 8, 2, [513, 900])):
+        B, T = len(lens), sum(lens)
+        pool = Pool(40 * B, 1, KV, hd, seed=hd)
+        work.append(dict(hd=hd, H=H, KV=KV, B=B, T=T, rows=rand(T, (H + 2 * KV) * hd).to(torch.bfloat16),
+                         cu=i32([0] + np.cumsum(lens).tolist()), pool=pool, q=rand(B, H, hd).to(torch.bfloat16),
+                         table=tables(np.random.default_rng(hd), [40] * B, 40 * B), ctx=i32([637 - 100 * b for b in range(B)]),
+                         logits=rand(70, 32000), stream=torch.cuda.Stream()))
+
+    def go(w):
+        H, KV, hd = w["H"], w["KV"], w["hd"]
+        q, k, v = w["rows"][:, :H * hd], w["rows"][:, H * hd:(H + KV) * hd], w["rows"][:, (H + KV) * hd:]
+        out = torch.zeros((w["T"], H * hd), dtype=q.dtype, device="cuda")
+        top, ids = torch.zeros((70, 4), device="cuda"), torch.zeros((70, 4), dtype=torch.int32, device="cuda")
+        rc = lib().nr_prompt_attention(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), out.data_ptr(),
+                                       out.stride(0), 1, w["cu"].data_ptr(), None, w["B"], w["T"], w["T"], H, KV, hd, None, stream())
+        rc |= lib().nr_token_logprobs(w["logits"].data_ptr(), 0, 32000, 70, 32000, None, 4, None, None, top.data_ptr(), ids.data_ptr(),
+                                      stream())
+        assert rc == 0
+        return out, decode(w["pool"], w["q"], w["table"], w["ctx"]), top, ids
+
+    want = [go(w) for w in work]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for i, w in enumerate(work):
+            with torch.cuda.stream(w["stream"]):
+                got.append((i, go(w)))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
